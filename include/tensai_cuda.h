@@ -421,6 +421,137 @@ TQ_EXPORT int tq_sample(const float *logits, int n, double temp, double u, int *
  * (seed, stream 3). A stand-in for a tokenized prompt. */
 TQ_EXPORT int tq_synth_tokens(int *out, int n, int vocab, uint64_t seed);
 
+/* ---- paged 8-bit key/value cache -------------------------------------------- */
+
+/* No counterpart in the reference, whose example loops keep one sequence's
+ * keys and values in float32 (_example/qwen/model.go:244-260): the cache of a
+ * process that serves several requests, or contexts for which float32 is too
+ * large. Positions live in pages of `page` tokens that any sequence may own;
+ * each (page, KV head) holds int8 codes and two float32 scales, one for its
+ * keys and one for its values: value = code * scale, |code| <= 127.
+ * n_layer, n_kv >= 1; hd (head size) a multiple of 8, at most 256; page 16,
+ * 32, 64 or 128 tokens; n_pages pages in all, of every layer alike (a page id
+ * names the same page in each layer). */
+typedef struct {
+    int n_layer, n_kv, hd, page, n_pages;
+} tq_kv_config;
+
+/* Creates a cache on the thread's current device (tq_set_device): all codes
+ * and scales zero. */
+TQ_EXPORT int tq_kv_create(const tq_kv_config *cfg, uint64_t *cache);
+/* Releases a cache (waits for the device first; a second call is a no-op). */
+TQ_EXPORT int tq_kv_free(uint64_t cache);
+
+/* Shape and device of a cache. Any output pointer may be NULL. */
+TQ_EXPORT int tq_kv_info(uint64_t cache, tq_kv_config *cfg, int *device);
+
+/* Problems that only the device sees (lengths, page ids and counts are device
+ * data): the kernels skip what they cannot do and set a bit. tq_kv_status
+ * waits for the cache's device, returns the bits and clears them. */
+#define TQ_KV_STATUS_POOL 1u   /* plan: too few free pages; release: free list full */
+#define TQ_KV_STATUS_TABLE 2u  /* a request needs more pages than its table row has */
+#define TQ_KV_STATUS_SLOTS 4u  /* plan: more new tokens than the slot array holds; store: a slot out of order */
+#define TQ_KV_STATUS_LENGTH 8u /* a negative length or count, or token starts that do not ascend */
+#define TQ_KV_STATUS_PAGE 16u  /* a page id or slot outside the cache */
+#define TQ_KV_STATUS_TIMEOUT 32u /* a kernel gave up a bounded wait: its output is invalid */
+TQ_EXPORT int tq_kv_status(uint64_t cache, unsigned *bits);
+
+/* The bookkeeping of one serving step; all arrays in device memory. Request i
+ * holds cached[i] tokens and brings added[i] new ones. Its row of the block
+ * table (table + i * table_stride, table_cols entries) names the pages of its
+ * positions, the first ceil(cached[i] / page) of which are valid. The call
+ *   takes the pages that the new tokens need from the top of the free list:
+ *     the j-th new page of the call (requests in order, positions in order) is
+ *     free_pages[*free_count - 1 - j]; *free_left = *free_count - their number;
+ *   writes them into the table, starts[0..n] = the exclusive sums of added
+ *     (starts[n] = all new tokens), lens[i] = cached[i] + added[i];
+ *   writes slots[t], the place of new token t (tokens of request 0, then 1, ..):
+ *     page id * page + offset; entries behind the last token stay as they were.
+ * free_left may be free_count, and lens may be cached; other arrays must not
+ * overlap. All or nothing: if anything does not fit, a status bit is set, no
+ * page is taken, starts are 0, lens = cached and slots[0..slots_cap) = -1, so
+ * that a store and an attention behind it do nothing. n <= TQ_KV_MAX_REQUESTS.
+ * One launch, asynchronous on stream; calls on one free list must not overlap. */
+#define TQ_KV_MAX_REQUESTS 16384
+typedef struct {
+    int n, table_stride, table_cols, free_cap, slots_cap;
+    const int *cached, *added;
+    int *table;
+    const int *free_pages, *free_count;
+    int *starts, *lens;
+    long long *slots;
+    int *free_left;
+} tq_kv_plan_args;
+TQ_EXPORT int tq_kv_plan_dev(uint64_t cache, const tq_kv_plan_args *args, void *stream);
+
+/* Puts the pages of every request with done[i] != 0 back on the free list
+ * (free_pages[*free_count + j], requests in order, pages in order) and sets its
+ * lens[i] to 0. free_left as in the plan. All or nothing: nothing changes when
+ * the list (free_cap entries) cannot take them or a length is bad. */
+typedef struct {
+    int n, table_stride, table_cols, free_cap;
+    const int *done;
+    int *lens;
+    const int *table;
+    int *free_pages;
+    const int *free_count;
+    int *free_left;
+} tq_kv_release_args;
+TQ_EXPORT int tq_kv_release_dev(uint64_t cache, const tq_kv_release_args *args, void *stream);
+
+/* Stores n new tokens of one layer: k and v are device arrays of n rows of
+ * [n_kv][hd] elements of type dtype (TQ_LINEAR_F32 / F16 / BF16), k_stride and
+ * v_stride elements apart; token t goes to slots[t] (negative: skipped). The
+ * tokens of one page must follow one another in ascending slots without a gap,
+ * as the plan writes them, and no page may occur twice otherwise.
+ * For each page and head, of the new tokens that fall into it: scale =
+ * float32(max|x| / 127); when positions before the first of them are held
+ * already, the larger of that and the present scale, and if it grew, the codes
+ * of those positions become round(code * old / new). New codes are
+ * round(x / scale). Both roundings are to the nearest integer of the exact
+ * quotient, ties to even. Positions behind the new tokens keep their codes. A
+ * maximum that is not finite makes the scale NaN, and with it every value of
+ * that page and head, until its first position is stored again. */
+TQ_EXPORT int tq_kv_store_dev(uint64_t cache, int layer, const void *k, const void *v, int dtype, long long k_stride,
+                              long long v_stride, const long long *slots, int n, void *stream);
+
+/* The attention of new tokens over the cache, one layer. q and out: n_tokens
+ * rows of [n_q][hd] elements of type dtype, q_stride and out_stride elements
+ * apart; query head h reads KV head h / (n_q / n_kv). Sequence i owns the rows
+ * starts[i] .. starts[i + 1] - 1, which are the last of its lens[i] positions:
+ * row j sees positions 0 .. lens[i] - (starts[i + 1] - starts[i]) + j (its own
+ * included) through row i of the table. out = softmax(scale * q . k) v; a row
+ * that sees nothing is 0; rows from starts[n] on stay as they were.
+ * workspace: tq_kv_attention_workspace bytes of device memory, 16-byte
+ * aligned, its first TQ_KV_WORKSPACE_HEAD bytes zero before the first call (each
+ * call leaves them zero) and never shared by two calls that may overlap (two
+ * streams, two graphs replayed at once); calls in order on one stream may share
+ * it. n <= TQ_KV_MAX_REQUESTS. Allocates nothing. */
+#define TQ_KV_WORKSPACE_HEAD 4096
+typedef struct {
+    const void *q;
+    void *out;
+    int dtype, n_q, n_tokens, n;
+    long long q_stride, out_stride;
+    const int *starts, *lens, *table;
+    int table_stride, table_cols;
+    float scale;
+    void *workspace;
+    size_t workspace_bytes;
+} tq_kv_attention_args;
+TQ_EXPORT int tq_kv_attention_workspace(uint64_t cache, size_t *bytes);
+TQ_EXPORT int tq_kv_attention_dev(uint64_t cache, int layer, const tq_kv_attention_args *args, void *stream);
+
+/* Pages in and out, for the n page ids in the device array pages: codes as
+ * [n][page][n_kv][hd] int8 and scales as [n][n_kv] float32 (load, save), or
+ * the values code * scale as [n][page][n_kv][hd] float32 (read). Device
+ * memory, asynchronous on stream. load clamps code -128 to -127. */
+TQ_EXPORT int tq_kv_load_dev(uint64_t cache, int layer, const int *pages, int n, const int8_t *k, const int8_t *v,
+                             const float *kscale, const float *vscale, void *stream);
+TQ_EXPORT int tq_kv_save_dev(uint64_t cache, int layer, const int *pages, int n, int8_t *k, int8_t *v, float *kscale,
+                             float *vscale, void *stream);
+TQ_EXPORT int tq_kv_read_dev(uint64_t cache, int layer, const int *pages, int n, float *k, float *v, void *stream);
+
 /* ---- host-side fault injection (tests) ------------------------------------ */
 
 /* Makes the next n device allocations made by this library fail with

@@ -76,6 +76,18 @@ SIGNATURES = {
     "tq_chain_run": (I, [U64, P]),
     "tq_chain_free": (I, [U64]),
     "tq_set_matvec_kernel": (I, [I]),
+    "tq_kv_create": (I, [P, PU64]),
+    "tq_kv_free": (I, [U64]),
+    "tq_kv_info": (I, [U64, P, PI]),
+    "tq_kv_status": (I, [U64, ctypes.POINTER(ctypes.c_uint)]),
+    "tq_kv_plan_dev": (I, [U64, P, P]),
+    "tq_kv_release_dev": (I, [U64, P, P]),
+    "tq_kv_store_dev": (I, [U64, I, P, P, I, ctypes.c_longlong, ctypes.c_longlong, P, I, P]),
+    "tq_kv_attention_workspace": (I, [U64, ctypes.POINTER(SZ)]),
+    "tq_kv_attention_dev": (I, [U64, I, P, P]),
+    "tq_kv_load_dev": (I, [U64, I, P, I, P, P, P, P, P]),
+    "tq_kv_save_dev": (I, [U64, I, P, I, P, P, P, P, P]),
+    "tq_kv_read_dev": (I, [U64, I, P, I, P, P, P]),
     "tq_debug_fail_allocs": (I, [I]),
 }
 
@@ -98,6 +110,46 @@ class ChainOp(ctypes.Structure):
     _fields_ = [("matrix", ctypes.c_uint64), ("x", ctypes.c_void_p), ("out", ctypes.c_void_p),
                 ("epilogue", ctypes.c_int), ("resid", ctypes.c_void_p), ("norm_w", ctypes.c_void_p),
                 ("norm_from", ctypes.c_int), ("eps", ctypes.c_double)]
+
+TQ_KV_STATUS_POOL = 1
+TQ_KV_STATUS_TABLE = 2
+TQ_KV_STATUS_SLOTS = 4
+TQ_KV_STATUS_LENGTH = 8
+TQ_KV_STATUS_PAGE = 16
+TQ_KV_STATUS_TIMEOUT = 32
+TQ_KV_WORKSPACE_HEAD = 4096
+TQ_KV_MAX_REQUESTS = 16384
+
+
+class KvConfig(ctypes.Structure):
+    """tq_kv_config of include/tensai_cuda.h."""
+
+    _fields_ = [(k, ctypes.c_int) for k in ("n_layer", "n_kv", "hd", "page", "n_pages")]
+
+
+class KvPlanArgs(ctypes.Structure):
+    """tq_kv_plan_args of include/tensai_cuda.h."""
+
+    _fields_ = ([(k, ctypes.c_int) for k in ("n", "table_stride", "table_cols", "free_cap", "slots_cap")] +
+                [(k, ctypes.c_void_p) for k in ("cached", "added", "table", "free_pages", "free_count", "starts",
+                                                "lens", "slots", "free_left")])
+
+
+class KvReleaseArgs(ctypes.Structure):
+    """tq_kv_release_args of include/tensai_cuda.h."""
+
+    _fields_ = ([(k, ctypes.c_int) for k in ("n", "table_stride", "table_cols", "free_cap")] +
+                [(k, ctypes.c_void_p) for k in ("done", "lens", "table", "free_pages", "free_count", "free_left")])
+
+
+class KvAttentionArgs(ctypes.Structure):
+    """tq_kv_attention_args of include/tensai_cuda.h."""
+
+    _fields_ = [("q", ctypes.c_void_p), ("out", ctypes.c_void_p), ("dtype", ctypes.c_int), ("n_q", ctypes.c_int),
+                ("n_tokens", ctypes.c_int), ("n", ctypes.c_int), ("q_stride", ctypes.c_longlong),
+                ("out_stride", ctypes.c_longlong), ("starts", ctypes.c_void_p), ("lens", ctypes.c_void_p),
+                ("table", ctypes.c_void_p), ("table_stride", ctypes.c_int), ("table_cols", ctypes.c_int),
+                ("scale", ctypes.c_float), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t)]
 
 
 class TensaiError(RuntimeError):
