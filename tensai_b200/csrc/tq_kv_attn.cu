@@ -28,23 +28,23 @@
 // data; every CTA makes the same sums). A warp's unfinished segments meet in its
 // CTA, the CTA's in the CTA that arrives last, in a fixed order: results do not
 // depend on timing.
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-#include <cuda_runtime.h>
+#include <climits>
 
-#include "tq_common.cuh"
-#include "tq_kv.h"
-#include "tq_ptx.cuh"
+#include "tq_kv_attn.cuh"
 
 namespace {
+
+using namespace tqkv;
+using Params = TqKvParams;
 
 constexpr int kTile = 64;       // positions per step of a warp
 constexpr int kSlots = 3;       // ring slots per warp
 constexpr int kMinTiles = 4;    // tiles per CTA below which fewer CTAs work
+constexpr int kPromptRows = 48; // rows of a sequence above which the prompt kernel takes it
 constexpr int kDirect = 1024;   // sequences whose lengths are kept in shared memory
-constexpr int kSums = 512;      // entries of the prefix sums
+constexpr int kSums = kKvSums;
 constexpr float kPUnit = 16384.f; // p = 1 in float16: its low piece stays normal
-constexpr size_t kHead = TQ_KV_WORKSPACE_HEAD; // workspace: arrival counters first
+constexpr size_t kHead = kKvHead;
 constexpr int kMaxGrid = kHead / sizeof(unsigned);
 
 constexpr int warps_of(int hdp) { return hdp == 256 ? 4 : 8; }
@@ -56,108 +56,6 @@ constexpr int partials_of(int hdp) { return 2 * warps_of(hdp) + 2; } // per CTA
 constexpr size_t smem_bytes(int hdp) {
     return (size_t)warps_of(hdp) * kSlots * slot_bytes(hdp) + sizeof(long long) * (kSums + 1) +
            sizeof(int) * (2 * kDirect + 2);
-}
-
-struct Params {
-    TqKvView c;
-    TqKvAttn a;
-    int group, vec, shift_sums; // prefix entry = 2^shift_sums sequences
-    float scale2;               // scale * log2(e)
-};
-
-struct Seq { // what a sequence's lengths say
-    int start, nq, len;
-};
-
-__device__ __forceinline__ void cvt4(unsigned w, unsigned &lo, unsigned &hi) {
-    // codes + 128 under the exponent of 1024, then minus 1152: exact
-    const unsigned u = w ^ 0x80808080u;
-    const unsigned a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
-    const __half2 off = __half2half2(__ushort_as_half(0x6480));
-    const __half2 x = __hsub2(*reinterpret_cast<const __half2 *>(&a), off);
-    const __half2 y = __hsub2(*reinterpret_cast<const __half2 *>(&b), off);
-    lo = *reinterpret_cast<const unsigned *>(&x);
-    hi = *reinterpret_cast<const unsigned *>(&y);
-}
-__device__ __forceinline__ unsigned pack2(float x, float y) {
-    const __half2 h = __floats2half2_rn(x, y);
-    return *reinterpret_cast<const unsigned *>(&h);
-}
-__device__ __forceinline__ float2 unpack2(unsigned u) { return __half22float2(*reinterpret_cast<const __half2 *>(&u)); }
-
-__device__ __forceinline__ void mma16816(float (&d)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-                 "{%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-template <typename T> struct Elem;
-template <> struct Elem<float> {
-    static __device__ __forceinline__ float get(const float *p) { return *p; }
-    static __device__ __forceinline__ void put2(float *p, float x, float y, bool vec, bool two) {
-        if (vec)
-            *reinterpret_cast<float2 *>(p) = make_float2(x, y);
-        else {
-            p[0] = x;
-            if (two) p[1] = y;
-        }
-    }
-};
-template <> struct Elem<__half> {
-    static __device__ __forceinline__ float get(const __half *p) { return __half2float(*p); }
-    static __device__ __forceinline__ void put2(__half *p, float x, float y, bool vec, bool two) {
-        if (vec)
-            *reinterpret_cast<__half2 *>(p) = __floats2half2_rn(x, y);
-        else {
-            p[0] = __float2half_rn(x);
-            if (two) p[1] = __float2half_rn(y);
-        }
-    }
-};
-template <> struct Elem<__nv_bfloat16> {
-    static __device__ __forceinline__ float get(const __nv_bfloat16 *p) { return __bfloat162float(*p); }
-    static __device__ __forceinline__ void put2(__nv_bfloat16 *p, float x, float y, bool vec, bool two) {
-        if (vec)
-            *reinterpret_cast<__nv_bfloat162 *>(p) = __floats2bfloat162_rn(x, y);
-        else {
-            p[0] = __float2bfloat16_rn(x);
-            if (two) p[1] = __float2bfloat16_rn(y);
-        }
-    }
-};
-
-// 8 consecutive elements, widened.
-template <typename T> __device__ __forceinline__ void load8(const T *p, bool vec, float (&x)[8]) {
-    if (vec) {
-        constexpr int E = 16 / sizeof(T);
-#pragma unroll
-        for (int j = 0; j < 8 / E; j++) {
-            const uint4 w = *reinterpret_cast<const uint4 *>(p + j * E);
-            const T *e = reinterpret_cast<const T *>(&w);
-#pragma unroll
-            for (int u = 0; u < E; u++) x[j * E + u] = Elem<T>::get(e + u);
-        }
-    } else {
-#pragma unroll
-        for (int u = 0; u < 8; u++) x[u] = Elem<T>::get(p + u);
-    }
-}
-
-// Bounded wait for a ring slot. A copy from mapped memory always arrives; should
-// one not, the status says so and no later wait of the CTA waits.
-__device__ __noinline__ void wait_long(uint64_t *bar, unsigned parity, volatile int *late, unsigned *status) {
-    const unsigned long long t0 = tqp::global_ns();
-    while (!*late) {
-        if (tqp::mbar_try_wait_hint(bar, parity, 200000u)) return;
-        if (tqp::global_ns() - t0 > tqp::kWaitNs) {
-            atomicOr(status, TQ_KV_STATUS_TIMEOUT);
-            *late = 1;
-        }
-    }
-}
-__device__ __forceinline__ void wait_slot(uint64_t *bar, unsigned parity, volatile int *late, unsigned *status) {
-    if (!tqp::mbar_try_wait(bar, parity)) wait_long(bar, parity, late, status);
 }
 
 template <int HDP, int PIECES, typename T>
@@ -188,19 +86,8 @@ __global__ void __launch_bounds__(32 * warps_of(HDP), ctas_of(HDP)) kv_attn_kern
     __syncthreads();
     const int *starts = direct ? s_starts : p.a.starts, *lens = direct ? s_lens : p.a.lens;
     auto seq_of = [&](int i) {
-        Seq s;
-        s.start = starts[i];
-        const int e = starts[i + 1];
-        s.nq = e - s.start;
-        s.len = lens[i];
-        if (s.start < 0 || e < s.start || e > p.a.n_tokens || s.len < 0) {
-            s.nq = s.len = 0;
-            atomicOr(p.c.status, TQ_KV_STATUS_LENGTH);
-        }
-        if (s.len > p.a.table_cols << p.c.page_shift) {
-            s.nq = s.len = 0;
-            atomicOr(p.c.status, TQ_KV_STATUS_TABLE);
-        }
+        Seq s = seq_at(p, starts, lens, i);
+        if (s.nq > p.rows_cut / group) s.nq = 0; // the prompt kernel's
         return s;
     };
     auto tiles_per = [](const Seq &s) { return s.len > kTile ? (s.len + kTile - 1) / kTile : 1; };
@@ -407,10 +294,7 @@ __global__ void __launch_bounds__(32 * warps_of(HDP), ctas_of(HDP)) kv_attn_kern
                         }
                     big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
                     big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
-                    // the row's largest magnitude to 2^13: float16 pieces keep their bits far below it
-                    const int ex = big > 0.f && big < INFINITY ? min(100, max(-100, 13 - ilogbf(big))) : 0;
-                    const float unit = ldexpf(1.f, ex);
-                    row_unit[h] = ldexpf(1.f, -ex);
+                    const float unit = row_scale(big, &row_unit[h]);
                     if (live) lim[h] = min(cur.s.len, max(0, cur.s.len - cur.s.nq + tok + 1));
 #pragma unroll
                     for (int kk = 0; kk < KK; kk++)
@@ -703,9 +587,13 @@ template <int HDP> cudaError_t launch_hd(const Params &p, int sms, cudaStream_t 
 
 } // namespace
 
-size_t tq_kv_attn_workspace(int hdp, int sms) {
+static size_t small_workspace(int hdp, int sms) {
     const size_t grid = (size_t)(sms * ctas_of(hdp) < kMaxGrid ? sms * ctas_of(hdp) : kMaxGrid);
     return kHead + grid * partials_of(hdp) * partial_floats(hdp) * sizeof(float);
+}
+size_t tq_kv_attn_workspace(int hdp, int sms) {
+    const size_t a = small_workspace(hdp, sms), b = tq_kv_prompt_workspace(hdp, sms);
+    return a > b ? a : b; // the two kernels of a call run one after the other
 }
 
 cudaError_t tq_kv_launch_attn(const TqKvView &v, const TqKvAttn &a, int sms, cudaStream_t st) {
@@ -720,6 +608,15 @@ cudaError_t tq_kv_launch_attn(const TqKvView &v, const TqKvAttn &a, int sms, cud
     p.shift_sums = 0;
     while ((a.n >> p.shift_sums) > kSums - 1) p.shift_sums++;
     p.scale2 = a.scale * 1.4426950408889634f;
+    p.rows_cut = INT_MAX;
+    // More tokens than sequences: some may bring enough rows for the tensor cores.
+    // (When others bring none, a long one can hide behind a small count; the
+    // kernel here then serves it too, in tiles of 8 or 16 rows.)
+    if (v.hdp <= 128 && (long long)(a.n_tokens - a.n + 1) * p.group > kPromptRows) {
+        p.rows_cut = kPromptRows;
+        const cudaError_t e = tq_kv_launch_prompt(p, sms, st);
+        if (e != cudaSuccess) return e;
+    }
     switch (v.hdp) {
     case 64: return launch_hd<64>(p, sms, st);
     case 128: return launch_hd<128>(p, sms, st);

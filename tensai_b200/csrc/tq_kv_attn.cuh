@@ -1,0 +1,163 @@
+// tq_kv_attn.cuh — what the two attention kernels over the paged 8-bit cache
+// share (tq_kv_attn.cu: few rows; tq_kv_prompt.cu: many).
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include "tq_common.cuh"
+#include "tq_kv.h"
+#include "tq_ptx.cuh"
+
+struct TqKvParams {
+    TqKvView c;
+    TqKvAttn a;
+    int group, vec, shift_sums; // prefix entry = 2^shift_sums sequences
+    int rows_cut;               // sequences of more rows (new tokens x group) are the prompt kernel's
+    float scale2;               // scale * log2(e)
+};
+constexpr int kKvSums = 512;                      // entries of the prefix sums
+constexpr size_t kKvHead = TQ_KV_WORKSPACE_HEAD; // workspace: arrival counters first
+
+namespace tqkv {
+
+struct Seq { // what a sequence's lengths say
+    int start, nq, len;
+};
+
+__device__ __forceinline__ void cvt4(unsigned w, unsigned &lo, unsigned &hi) {
+    // codes + 128 under the exponent of 1024, then minus 1152: exact
+    const unsigned u = w ^ 0x80808080u;
+    const unsigned a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
+    const __half2 off = __half2half2(__ushort_as_half(0x6480));
+    const __half2 x = __hsub2(*reinterpret_cast<const __half2 *>(&a), off);
+    const __half2 y = __hsub2(*reinterpret_cast<const __half2 *>(&b), off);
+    lo = *reinterpret_cast<const unsigned *>(&x);
+    hi = *reinterpret_cast<const unsigned *>(&y);
+}
+__device__ __forceinline__ unsigned pack2(float x, float y) {
+    const __half2 h = __floats2half2_rn(x, y);
+    return *reinterpret_cast<const unsigned *>(&h);
+}
+__device__ __forceinline__ float2 unpack2(unsigned u) { return __half22float2(*reinterpret_cast<const __half2 *>(&u)); }
+
+__device__ __forceinline__ void mma16816(float (&d)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+                 "{%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+template <typename T> struct Elem;
+template <> struct Elem<float> {
+    static __device__ __forceinline__ float get(const float *p) { return *p; }
+    static __device__ __forceinline__ void put2(float *p, float x, float y, bool vec, bool two) {
+        if (vec)
+            *reinterpret_cast<float2 *>(p) = make_float2(x, y);
+        else {
+            p[0] = x;
+            if (two) p[1] = y;
+        }
+    }
+};
+template <> struct Elem<__half> {
+    static __device__ __forceinline__ float get(const __half *p) { return __half2float(*p); }
+    static __device__ __forceinline__ void put2(__half *p, float x, float y, bool vec, bool two) {
+        if (vec)
+            *reinterpret_cast<__half2 *>(p) = __floats2half2_rn(x, y);
+        else {
+            p[0] = __float2half_rn(x);
+            if (two) p[1] = __float2half_rn(y);
+        }
+    }
+};
+template <> struct Elem<__nv_bfloat16> {
+    static __device__ __forceinline__ float get(const __nv_bfloat16 *p) { return __bfloat162float(*p); }
+    static __device__ __forceinline__ void put2(__nv_bfloat16 *p, float x, float y, bool vec, bool two) {
+        if (vec)
+            *reinterpret_cast<__nv_bfloat162 *>(p) = __floats2bfloat162_rn(x, y);
+        else {
+            p[0] = __float2bfloat16_rn(x);
+            if (two) p[1] = __float2bfloat16_rn(y);
+        }
+    }
+};
+
+// 8 consecutive elements, widened.
+template <typename T> __device__ __forceinline__ void load8(const T *p, bool vec, float (&x)[8]) {
+    if (vec) {
+        constexpr int E = 16 / sizeof(T);
+#pragma unroll
+        for (int j = 0; j < 8 / E; j++) {
+            const uint4 w = *reinterpret_cast<const uint4 *>(p + j * E);
+            const T *e = reinterpret_cast<const T *>(&w);
+#pragma unroll
+            for (int u = 0; u < E; u++) x[j * E + u] = Elem<T>::get(e + u);
+        }
+    } else {
+#pragma unroll
+        for (int u = 0; u < 8; u++) x[u] = Elem<T>::get(p + u);
+    }
+}
+
+// 8 consecutive elements, rounded.
+template <typename T> __device__ __forceinline__ void store8(T *p, bool vec, const float (&x)[8]) {
+    if (vec) {
+        __align__(16) T e[8];
+#pragma unroll
+        for (int u = 0; u < 8; u += 2) Elem<T>::put2(e + u, x[u], x[u + 1], true, true);
+#pragma unroll
+        for (int j = 0; j < (int)sizeof(e) / 16; j++) reinterpret_cast<uint4 *>(p)[j] = reinterpret_cast<const uint4 *>(e)[j];
+    } else {
+#pragma unroll
+        for (int u = 0; u < 8; u += 2) Elem<T>::put2(p + u, x[u], x[u + 1], false, true);
+    }
+}
+
+// A sequence's lengths, checked: one that cannot be served has no tokens.
+__device__ __forceinline__ Seq seq_at(const TqKvParams &p, const int *starts, const int *lens, int i) {
+    Seq s;
+    s.start = starts[i];
+    const int e = starts[i + 1];
+    s.nq = e - s.start;
+    s.len = lens[i];
+    if (s.start < 0 || e < s.start || e > p.a.n_tokens || s.len < 0) {
+        s.nq = s.len = 0;
+        atomicOr(p.c.status, TQ_KV_STATUS_LENGTH);
+    }
+    if (s.len > p.a.table_cols << p.c.page_shift) {
+        s.nq = s.len = 0;
+        atomicOr(p.c.status, TQ_KV_STATUS_TABLE);
+    }
+    return s;
+}
+
+// Bounded wait for an mbarrier. What it waits for always arrives; should it not, the status says so and no later wait of the CTA waits.
+static __device__ __noinline__ void wait_long(uint64_t *bar, unsigned parity, volatile int *late, unsigned *status) {
+    const unsigned long long t0 = tqp::global_ns();
+    while (!*late) {
+        if (tqp::mbar_try_wait_hint(bar, parity, 200000u)) return;
+        if (tqp::global_ns() - t0 > tqp::kWaitNs) {
+            atomicOr(status, TQ_KV_STATUS_TIMEOUT);
+            *late = 1;
+        }
+    }
+}
+__device__ __forceinline__ void wait_slot(uint64_t *bar, unsigned parity, volatile int *late, unsigned *status) {
+    if (!tqp::mbar_try_wait(bar, parity)) wait_long(bar, parity, late, status);
+}
+
+// The power of two that brings a row's largest magnitude to 2^13: float16 pieces
+// keep their bits far below it. *back: its inverse.
+__device__ __forceinline__ float row_scale(float big, float *back) {
+    const int ex = big > 0.f && big < INFINITY ? min(100, max(-100, 13 - ilogbf(big))) : 0;
+    *back = ldexpf(1.f, -ex);
+    return ldexpf(1.f, ex);
+}
+
+} // namespace tqkv
+
+// Many rows a sequence on the tensor cores; hdp 64 or 128 (tq_kv_prompt.cu).
+size_t tq_kv_prompt_workspace(int hdp, int sms);
+cudaError_t tq_kv_launch_prompt(const TqKvParams &p, int sms, cudaStream_t st);

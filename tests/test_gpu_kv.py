@@ -332,20 +332,23 @@ def batch(rng, n_kv, hd, page, lens, extra=3, wide=1.0):
     return cache, ref, table
 
 
-def bound(ref_out, mag, qk, top_v, dtype, hd, group, longest):
+def bound(ref_out, mag, qk, top_v, dtype, hd, group, longest, new):
     """What the arithmetic allows. Per position: the score's hd products (22 bits
     of q, float32 sums that the tensor cores may truncate: 2^-22 each) move p by
     twice their error; exp2 and the pieces of p 2^-21; 2^-12 where p is one
-    float16 (16-bit queries, more than eight heads to a KV head); every addition
-    over the positions 2^-22; then the output's own rounding.
+    float16 (16-bit queries, more than eight heads to a KV head or many rows);
+    every addition over the positions 2^-22; then the output's own rounding.
     p times its value scale, over the largest value scale, is held in float16 at
     2^14 for p = 1, whose steps below 2^-14 are 2^-24: a rounding of at most
     2^-25 / 2^14 = 2^-39 of the largest value for each position, whatever p is
-    (after division by the sum of p, which is at least 1)."""
-    one = dtype != "f32" and group > 8
+    (after division by the sum of p, which is at least 1). With many rows the
+    unit is 2^10 for the largest p times its scale, or up to 2^4 below that:
+    2^-25 / 2^10 = 2^-35."""
+    many = max(new, default=0) * group > 48 and hd <= 128  # the tensor-memory kernel
+    one = dtype != "f32" and (group > 8 or many)
     rel = 2 * (hd + 16) * 2.0**-22 * qk + (longest + 64) * 2.0**-22 + 2.0**-21 + (2.0**-11 if one else 0)
     half = torch.finfo(DT[dtype]).eps / 2
-    floor = longest * 2.0**-39 * top_v
+    floor = longest * (2.0**-35 if many else 2.0**-39) * top_v
     return mag * rel[..., None] + floor[..., None] + np.abs(ref_out) * half * 1.0001 + 2.0**-24 * half
 
 
@@ -358,7 +361,7 @@ def run_attention(cache, ref, table, lens, new, dtype, n_q, rng, scale=None, q_s
     want, mag, qk, top_v = ref.attention(np_(q), starts, lens, table, hd**-0.5 if scale is None else scale)
     got = np_(out)
     assert np.all(got[T:] == 7)
-    tol = bound(want, mag, qk, top_v, dtype, hd, n_q // ref.n_kv, max(lens, default=0))
+    tol = bound(want, mag, qk, top_v, dtype, hd, n_q // ref.n_kv, max(lens, default=0), new)
     err = np.abs(got - want)[:T]
     assert np.all(err <= tol[:T]), (float(np.max(err - tol[:T])), float(np.max(err)))
     return q, out
@@ -543,7 +546,7 @@ def test_offsets_beyond_32_bits():
         q = torch.tensor(rng.standard_normal((2, n_kv, hd)), device="cuda", dtype=torch.float32)
         out = cache.attention(0, q, cu([0, 2]), cu([200]), cu([ids]))
         want, mag, qk, top_v = small.attention(np_(q), [0, 2], [200], np.array([[0, 1]]), hd**-0.5)
-        assert np.all(np.abs(np_(out) - want) <= bound(want, mag, qk, top_v, "f32", hd, 1, 200))
+        assert np.all(np.abs(np_(out) - want) <= bound(want, mag, qk, top_v, "f32", hd, 1, 200, [2]))
         cache.check()
 
 
@@ -574,7 +577,7 @@ def test_a_serving_run():
             ref.store(np_(k)[:T], np_(v)[:T], w_slots)
             out = cache.attention(0, q, starts, lens, table)
             want, mag, qk, top_v = ref.attention(np_(q)[:T], w_starts, w_lens, w_table, hd**-0.5)
-            assert np.all(np.abs(np_(out)[:T] - want) <= bound(want, mag, qk, top_v, "f32", hd, 3, 60))
+            assert np.all(np.abs(np_(out)[:T] - want) <= bound(want, mag, qk, top_v, "f32", hd, 3, 60, list(added)))
             if step % 4 == 3:
                 cache.release(cu((rng.random(n) < 0.5).astype(int)), lens, table, free, count)
         cache.check()
