@@ -134,7 +134,7 @@ __device__ __forceinline__ Seq seq_at(const TqKvParams &p, const int *starts, co
 }
 
 // Bounded wait for an mbarrier. What it waits for always arrives; should it not, the status says so and no later wait of the CTA waits.
-static __device__ __noinline__ void wait_long(uint64_t *bar, unsigned parity, volatile int *late, unsigned *status) {
+__device__ __forceinline__ void wait_long(uint64_t *bar, unsigned parity, volatile int *late, unsigned *status) {
     const unsigned long long t0 = tqp::global_ns();
     while (!*late) {
         if (tqp::mbar_try_wait_hint(bar, parity, 200000u)) return;
@@ -148,12 +148,13 @@ __device__ __forceinline__ void wait_slot(uint64_t *bar, unsigned parity, volati
     if (!tqp::mbar_try_wait(bar, parity)) wait_long(bar, parity, late, status);
 }
 
-// The power of two that brings a row's largest magnitude to 2^13: float16 pieces
-// keep their bits far below it. *back: its inverse.
+// The power of two that brings a row's largest magnitude to 2^13 .. 2^14: float16
+// pieces keep their bits far below it (magnitudes under 2^-87 count as 2^-87).
+// *back: its inverse.
 __device__ __forceinline__ float row_scale(float big, float *back) {
-    const int ex = big > 0.f && big < INFINITY ? min(100, max(-100, 13 - ilogbf(big))) : 0;
-    *back = ldexpf(1.f, -ex);
-    return ldexpf(1.f, ex);
+    const int e = max(40, (int)(__float_as_uint(big) >> 23)); // its exponent + 127; 255 for an infinity
+    *back = __uint_as_float((unsigned)(e - 13) << 23);
+    return __uint_as_float((unsigned)(267 - e) << 23);
 }
 
 } // namespace tqkv

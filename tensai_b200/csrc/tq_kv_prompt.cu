@@ -42,64 +42,54 @@ constexpr int kPos = 128;       // positions of a tile
 constexpr int kBlocks = kPos / TQ_KV_BLOCK;
 constexpr int kSoftWarps = 8, kConvWarps = 4;
 constexpr int kConvThreads = 32 * kConvWarps;
-constexpr int kMmaWarp = kSoftWarps + kConvWarps; // one thread of it issues
-constexpr int kThreads = 32 * (kMmaWarp + 1);
+constexpr int kMmaWarp = kSoftWarps + kConvWarps; // one thread of it issues; the next warp loads
+constexpr int kThreads = 32 * (kMmaWarp + 4);      // four warpgroups, for the split of the registers:
+// softmax (a row of S stays in registers), widening, the rest.
+constexpr int soft_regs(int pieces) { return pieces == 1 ? 192 : 176; }
+constexpr int conv_regs(int pieces) { return pieces == 1 ? 64 : 72; }
+constexpr int mma_regs(int pieces) { return pieces == 1 ? 64 : 88; }
+static_assert(2 * soft_regs(1) + conv_regs(1) + mma_regs(1) <= 4 * 128, "no more than the launch's registers");
+static_assert(2 * soft_regs(2) + conv_regs(2) + mma_regs(2) <= 4 * 128, "no more than the launch's registers");
 constexpr int kConsts = 4;      // position tiles whose scales are kept
 constexpr int kMinTiles = 2;    // position tiles per CTA below which fewer CTAs work
 constexpr float kSlack = 4.f;   // log2 by which w may exceed M
 constexpr float kUnit = 10.f;   // log2 of P at w = M
+constexpr float kLeast = 1e-30f; // least score factor of a block: -inf times it stays -inf
 constexpr int kJoinThreads = 256, kJoinRows = 32;
 
 constexpr int stages_of(int hdp, int pieces) { return hdp == 128 && pieces == 2 ? 1 : 2; }
 constexpr size_t operand_bytes(int hdp) { return (size_t)kPos * hdp * 2; } // a K or V tile, or a piece of a Q tile
 constexpr size_t smem_bytes(int hdp, int pieces) {
-    return 1024 + operand_bytes(hdp) * (2 * pieces + 2 * stages_of(hdp, pieces)) + sizeof(long long) * (kKvSums + 1);
+    return 1024 + operand_bytes(hdp) * (2 * pieces + 2 * stages_of(hdp, pieces) + 1); // the staged codes are one more
 }
 constexpr size_t partial_floats(int hdp) { return (size_t)kBlockRows * (hdp + 2); }
 
 // ---- the list of work ------------------------------------------------------------------
 
-// sum of floor((a i + b) / m) for i < n (a, b >= 0): the points under a line,
-// counted by the Euclidean algorithm.
-__device__ __forceinline__ long long floor_sum(long long n, long long m, long long a, long long b) {
-    long long s = 0;
-    while (n > 0) {
-        s += (a / m) * (n * (n - 1) / 2) + (b / m) * n;
-        a %= m;
-        b %= m;
-        const long long top = a * n + b;
-        if (top < m) break;
-        n = top / m;
-        b = top % m;
-        const long long t = m;
-        m = a;
-        a = t;
-    }
-    return s;
-}
-
-// A sequence's row blocks: block rb has tiles(rb) position tiles,
-// floor((step rb + base) / div) but for the last block.
+// A sequence's row blocks. Block rb's last row is of new token (256 rb + 255) /
+// group, so it sees `first` + that many positions; the last block sees them all.
 struct Blocks {
     int nrb, last;
-    long long step, base, div;
-    __device__ __forceinline__ int tiles(int rb) const {
-        return rb == nrb - 1 ? last : (int)((step * rb + base) / div);
+    unsigned first; // 0: every block like the last (some rows see nothing)
+    __device__ __forceinline__ int tiles(int rb, int group) const {
+        if (rb == nrb - 1 || first == 0) return last;
+        return (int)((first + (unsigned)(rb * kBlockRows + kBlockRows - 1) / (unsigned)group + kPos - 1) / kPos);
     }
-    __device__ __forceinline__ long long before(int rb) const { return floor_sum(min(rb, nrb - 1), div, step, base) + (rb == nrb ? last : 0); }
 };
 __device__ __forceinline__ Blocks blocks_of(const Seq &s, int group) {
     Blocks b;
-    b.nrb = (int)(((long long)s.nq * group + kBlockRows - 1) / kBlockRows);
-    b.last = max(1, (s.len + kPos - 1) / kPos);
-    if (s.nq > s.len) { // some rows see nothing: every block as long as the last
-        b.step = 0, b.base = b.last, b.div = 1;
-    } else { // its last row's position, + 1: len - nq + 1 + floor((256 rb + 255) / group)
-        b.step = kBlockRows;
-        b.base = (long long)(s.len - s.nq + 1) * group + kBlockRows - 1 + (long long)(kPos - 1) * group;
-        b.div = (long long)kPos * group;
-    }
+    b.nrb = (s.nq * group + kBlockRows - 1) / kBlockRows;
+    b.last = max(1, (int)(((unsigned)s.len + kPos - 1) / kPos));
+    b.first = s.nq > s.len ? 0u : (unsigned)(s.len - s.nq + 1);
     return b;
+}
+// The position tiles of one head, by a whole warp.
+__device__ __forceinline__ long long head_tiles(const Blocks &b, int group) {
+    long long t = 0;
+    for (int rb = threadIdx.x & 31; rb < b.nrb; rb += 32) t += b.tiles(rb, group);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+    return t;
 }
 
 struct Where { // a segment and a position tile of it
@@ -121,18 +111,32 @@ template <int NT> __device__ __forceinline__ long long list_sums(const Params &p
     __shared__ long long scan[NW];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int n = p.a.n, entries = (n + (1 << p.shift_sums) - 1) >> p.shift_sums;
+    for (int e = tid; e < entries; e += NT) sums[e] = 0;
+    __syncthreads();
+    // 32 sequences a turn, a lane each; those of several blocks by the whole warp
+    for (int i0 = warp * 32; i0 < n; i0 += NT) {
+        const int i = i0 + lane;
+        Seq s{0, 0, 0};
+        if (i < n) s = prompt_seq(p, i);
+        const Blocks b = blocks_of(s, p.group);
+        long long t = s.nq && b.nrb == 1 ? b.tiles(0, p.group) : 0;
+        for (unsigned many = __ballot_sync(0xffffffffu, s.nq && b.nrb > 1); many; many &= many - 1) {
+            const int l = __ffs(many) - 1;
+            const Blocks o = {__shfl_sync(0xffffffffu, b.nrb, l), __shfl_sync(0xffffffffu, b.last, l),
+                              __shfl_sync(0xffffffffu, b.first, l)};
+            const long long all = head_tiles(o, p.group);
+            if (lane == l) t = all;
+        }
+        if (t)
+            atomicAdd(reinterpret_cast<unsigned long long *>(sums + (i >> p.shift_sums)),
+                      (unsigned long long)(t * p.c.n_kv));
+    }
+    __syncthreads();
     long long own[PER], sum = 0;
 #pragma unroll
     for (int u = 0; u < PER; u++) {
         const int e = tid * PER + u;
-        own[u] = 0;
-        if (e < entries)
-            for (int i = e << p.shift_sums; i < min(n, (e + 1) << p.shift_sums); i++) {
-                const Seq s = prompt_seq(p, i);
-                if (s.nq == 0) continue;
-                const Blocks b = blocks_of(s, p.group);
-                own[u] += b.before(b.nrb) * p.c.n_kv;
-            }
+        own[u] = e < entries ? sums[e] : 0;
         sum += own[u];
     }
     long long inc = sum;
@@ -174,30 +178,37 @@ __device__ __forceinline__ Where find(const Params &p, const long long *sums, lo
         else
             hi = mid;
     }
-    long long rest = x - sums[lo], per = 0;
+    long long rest = x - sums[lo];
+    w.head = 0;
     for (w.i = lo << p.shift_sums; w.i < p.a.n; w.i++) {
         w.s = prompt_seq(p, w.i);
         if (w.s.nq == 0) continue;
         w.b = blocks_of(w.s, p.group);
-        per = w.b.before(w.b.nrb);
-        if (rest < per * p.c.n_kv) break;
+        const long long per = head_tiles(w.b, p.group);
+        if (rest < per * p.c.n_kv) {
+            for (; rest >= per; rest -= per) w.head++;
+            break;
+        }
         rest -= per * p.c.n_kv;
     }
-    w.head = (int)(rest / per);
-    rest -= per * w.head;
-    // the last row block that starts at or before `rest`: 32 candidates at a time
-    int a = 0, z = w.b.nrb; // before(a) <= rest < before(z)
-    while (z - a > 1) {
-        const int stride = (z - a + 31) / 32, c = min(z, a + lane * stride);
-        const unsigned ok = __ballot_sync(0xffffffffu, w.b.before(c) <= rest);
-        const int k = 31 - __clz(ok);
-        const int na = min(z, a + k * stride);
-        z = min(z, na + stride);
-        a = na;
+    for (int r0 = 0;; r0 += 32) { // 32 row blocks at a time
+        const int mine = r0 + lane < w.b.nrb ? w.b.tiles(r0 + lane, p.group) : 0;
+        long long upto = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long v = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += v;
+        }
+        const unsigned beyond = __ballot_sync(0xffffffffu, upto > rest);
+        if (beyond || r0 + 32 >= w.b.nrb) {
+            const int l = beyond ? __ffs(beyond) - 1 : 31;
+            w.rb = r0 + l;
+            w.tiles = __shfl_sync(0xffffffffu, mine, l);
+            w.tile = (int)(rest - (__shfl_sync(0xffffffffu, upto, l) - w.tiles));
+            break;
+        }
+        rest -= __shfl_sync(0xffffffffu, upto, 31);
     }
-    w.rb = a;
-    w.tile = (int)(rest - w.b.before(a));
-    w.tiles = w.b.tiles(a);
     w.from = x - w.tile;
     return w;
 }
@@ -217,7 +228,7 @@ __device__ __forceinline__ void next_segment(const Params &p, Where &w) {
             w.b = blocks_of(w.s, p.group);
         }
     }
-    w.tiles = w.b.tiles(w.rb);
+    w.tiles = w.b.tiles(w.rb, p.group);
 }
 
 // Positions that row `row` of the sequence sees.
@@ -242,16 +253,6 @@ __device__ __forceinline__ void tmem_ld32(uint32_t a, uint32_t (&v)[32]) {
           "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]),
           "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
         : "r"(a)
-        : "memory");
-}
-__device__ __forceinline__ void tmem_st32(uint32_t a, const uint32_t (&v)[32]) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
-        "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(a),
-        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
-        "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]),
-        "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]),
-        "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
         : "memory");
 }
 __device__ __forceinline__ void tmem_st16(uint32_t a, const uint32_t (&v)[16]) {
@@ -290,10 +291,33 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
+constexpr int kSegs = 4; // segments known ahead
+
+// A segment as the loader hands it to the other roles.
+struct Seg {
+    int start, nq, len; // the sequence: first token, tokens, positions
+    int head, row0;     // KV head, first row
+    int tile, cnt;      // position tiles tile .. tile + cnt - 1 here; cnt = 0: no more segments
+    int mine[2];        // of those, how many row tiles A and B see
+    int part;           // -1: the whole segment; else the workspace part
+};
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float y;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    return y;
+}
+
 struct Shared { // static shared memory
+    uint64_t seg_full[kSegs], seg_empty[kSegs];
+    uint64_t code_full[2], code_empty[2]; // staged codes: keys, values
     uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
     uint64_t q_ready[2], s_full[2], p_ready[2], o_full[2];
+    Seg seg[kSegs];
     float f[kConsts][kBlocks], lv[kConsts][kBlocks], rv[kConsts][kBlocks];
+    unsigned poison[kConsts]; // blocks with a scale that is not a number
+    float back[2][kRows]; // what a row of Q was divided by
+    unsigned live[2]; // blocks of the staged keys, values that are there (values: and not all zero)
     uint32_t tmem;
     volatile int late;
 };
@@ -301,24 +325,29 @@ struct Shared { // static shared memory
 template <int HDP, int PIECES, typename T>
 __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const __grid_constant__ Params p) {
     constexpr int ST = stages_of(HDP, PIECES);
-    constexpr uint32_t OP = (uint32_t)operand_bytes(HDP);
+    constexpr uint32_t OP = (uint32_t)operand_bytes(HDP), CODES = (uint32_t)kPos * HDP;
     extern __shared__ unsigned char raw[];
     __shared__ __align__(16) Shared sh;
     unsigned char *base = reinterpret_cast<unsigned char *>(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
-    unsigned char *Qs = base;                       // [2 tiles][PIECES][OP]
-    unsigned char *Ks = Qs + 2 * PIECES * OP;       // [ST][OP]
-    unsigned char *Vs = Ks + ST * OP;               // [ST][OP]
-    long long *sums = reinterpret_cast<long long *>(Vs + ST * OP);
+    unsigned char *Qs = base;                 // [2 tiles][PIECES][OP]
+    unsigned char *Ks = Qs + 2 * PIECES * OP; // [ST][OP]
+    unsigned char *Vs = Ks + ST * OP;         // [ST][OP]
+    unsigned char *Cs = Vs + ST * OP;         // [keys, values][CODES]: as the cache holds them
+    long long *sums = reinterpret_cast<long long *>(Cs); // before the first codes
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int group = p.group;
     const long long total = list_sums<kThreads>(p, sums);
     const int G = (int)min((long long)gridDim.x, (total + kMinTiles - 1) / kMinTiles);
     if ((int)blockIdx.x >= G) return; // none: G = 0
-    const TqSplit split(total, G);
-    const long long x0 = split.start(blockIdx.x), x1 = split.start(blockIdx.x + 1);
 
     if (tid == 0) {
+        for (int s = 0; s < kSegs; s++) {
+            tqp::mbar_init(&sh.seg_full[s], 1);
+            tqp::mbar_init(&sh.seg_empty[s], kSoftWarps + kConvWarps + 1);
+        }
         for (int s = 0; s < 2; s++) {
+            tqp::mbar_init(&sh.code_full[s], 1);
+            tqp::mbar_init(&sh.code_empty[s], kConvWarps);
             tqp::mbar_init(&sh.k_full[s], kConvThreads);
             tqp::mbar_init(&sh.v_full[s], kConvThreads);
             tqp::mbar_init(&sh.k_empty[s], 1);
@@ -344,127 +373,162 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const __grid_con
     // columns: S of A, S of B (P over them), O of A, O of B
     auto s_col = [&](int t) { return tmem + t * kPos; };
     auto o_col = [&](int t) { return tmem + 2 * kPos + t * HDP; };
-
-    Where w = find(p, sums, x0);
-    long long x = x0; // position tiles of the list done
+    auto next_seg = [&](unsigned n) -> const Seg & {
+        wait_slot(&sh.seg_full[n % kSegs], (n / kSegs) & 1, &sh.late, p.c.status);
+        return sh.seg[n % kSegs];
+    };
 
     if (warp < kSoftWarps) {
         // ================= softmax: thread = row of tile t =================
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(soft_regs(PIECES)));
         const int t = warp >> 2, row = (warp & 3) * 32 + lane;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t s_at = s_col(t) + lanes, o_at = o_col(t) + lanes;
         unsigned tick = 0, s_phase = 0, o_phase = 0; // position tiles of the CTA so far; barrier phases
-        while (x < x1) {
-            const int cnt = (int)min((long long)(w.tiles - w.tile), x1 - x);
-            const int mine = min(cnt, max(0, tiles_of(w, t, group) - w.tile));
-            const int rows = w.s.nq * group, r = w.rb * kBlockRows + t * kRows + row;
-            const int tok = r / group, hq = w.head * group + r - tok * group;
-            const bool live = r < rows;
-            const int lim = live ? sees(w.s, r, group) : w.s.len;
+        for (unsigned n = 0;; n++) {
+            const Seg &g = next_seg(n);
+            const int cnt = g.cnt, mine = g.mine[t], tile0 = g.tile, part_at = g.part;
+            if (cnt == 0) break;
+            const int row0 = g.row0, head = g.head, start = g.start, rows = g.nq * group;
+            const int r = row0 + t * kRows + row;
+            const int len = g.len, fresh = g.nq;
+            __syncwarp();
+            if (lane == 0) tqp::mbar_arrive(&sh.seg_empty[n % kSegs]);
+            // the row's place among the queries and the outputs, -1 for a row that is not there
+            const int tok = r / group, hq = head * group + r - tok * group;
+            const long long q_at = r < rows ? (long long)(start + tok) * p.a.q_stride + (long long)hq * p.c.hd : -1;
+            const long long o_at_row = r < rows ? (long long)(start + tok) * p.a.out_stride + (long long)hq * p.c.hd : -1;
+            const int lim = r < rows ? min(len, max(0, len - fresh + tok + 1)) : len;
             float M = -INFINITY, L = 0.f;
             if (mine > 0) {
-                // ---- this row of Q, as float16 pieces ----
-                const T *q = static_cast<const T *>(p.a.q) + (size_t)(w.s.start + tok) * p.a.q_stride + (size_t)hq * p.c.hd;
-                float big = 0.f;
-                for (int d = 0; d < HDP; d += 8) {
-                    float y[8];
-                    if (live && d < p.c.hd) {
-                        load8(q + d, p.vec, y);
-#pragma unroll
-                        for (int u = 0; u < 8; u++) big = fmaxf(big, fabsf(y[u]));
-                    }
-                }
-                float back;
-                float unit = row_scale(big, &back);
-                if (p.scale2 < 0.f) unit = -unit; // the block factors stay positive
+                // ---- Q, as float16 pieces: the warp's 32 rows, each by as many lanes as it has 16-byte words ----
+                constexpr int E = 16 / sizeof(T), LANES = HDP / E, ROWS = 32 / LANES;
                 unsigned char *qs = Qs + t * PIECES * OP;
-                for (int c = 0; c < HDP / 8; c++) {
-                    float y[8];
-                    if (live && 8 * c < p.c.hd)
-                        load8(q + 8 * c, p.vec, y);
-                    else
+                const int d = (lane % LANES) * E;
+                constexpr int BATCH = 8; // words in flight
+#pragma unroll 1
+                for (int i0 = 0; i0 < 32 / ROWS; i0 += BATCH) {
+                    uint4 word[BATCH];
+                    const T *from[BATCH];
 #pragma unroll
-                        for (int u = 0; u < 8; u++) y[u] = 0.f;
-                    unsigned hi[4], lo[4];
+                    for (int u = 0; u < BATCH; u++) {
+                        const int sr = (i0 + u) * ROWS + lane / LANES;
+                        const long long at = __shfl_sync(0xffffffffu, q_at, sr & 31);
+                        from[u] = sr < 32 && at >= 0 && d < p.c.hd ? static_cast<const T *>(p.a.q) + at + d : nullptr;
+                    }
+                    if (p.vec) {
 #pragma unroll
-                    for (int u = 0; u < 4; u++) {
+                        for (int u = 0; u < BATCH; u++)
+                            word[u] = from[u] ? __ldg(reinterpret_cast<const uint4 *>(from[u])) : make_uint4(0, 0, 0, 0);
+                    } else {
+#pragma unroll
+                        for (int u = 0; u < BATCH; u++)
+#pragma unroll
+                            for (int e = 0; e < E; e++) reinterpret_cast<T *>(&word[u])[e] = from[u] ? from[u][e] : T(0.f);
+                    }
+#pragma unroll
+                for (int i = 0; i < BATCH; i++) {
+                    if (i0 + i >= 32 / ROWS) break;
+                    const int qrow = (warp & 3) * 32 + (i0 + i) * ROWS + lane / LANES;
+                    float y[E];
+#pragma unroll
+                    for (int e = 0; e < E; e++) y[e] = Elem<T>::get(reinterpret_cast<const T *>(&word[i]) + e);
+                    float big = 0.f, was;
+#pragma unroll
+                    for (int u = 0; u < E; u++) big = fmaxf(big, fabsf(y[u]));
+#pragma unroll
+                    for (int o = 1; o < LANES; o <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+                    float unit = row_scale(big, &was);
+                    if (p.scale2 < 0.f) unit = -unit; // the block factors stay positive
+                    if (lane % LANES == 0) sh.back[t][qrow] = was;
+                    unsigned hi[E / 2], lo[E / 2];
+#pragma unroll
+                    for (int u = 0; u < E / 2; u++) {
                         const float a = y[2 * u] * unit, b = y[2 * u + 1] * unit;
                         hi[u] = pack2(a, b);
                         const float2 h = unpack2(hi[u]);
                         lo[u] = pack2(a - h.x, b - h.y);
                     }
-                    const uint32_t at = (c >> 3) * (kRows * 128) + chunk_at(row, c & 7);
-                    *reinterpret_cast<uint4 *>(qs + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                    if (PIECES == 2) *reinterpret_cast<uint4 *>(qs + OP + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                    unsigned char *to = qs + (d >> 6) * (kRows * 128) + chunk_at(qrow, (d & 63) >> 3) + 2 * (d & 7);
+                    if (E == 8) {
+                        *reinterpret_cast<uint4 *>(to) = make_uint4(hi[0], hi[1], hi[E / 2 - 2], hi[E / 2 - 1]);
+                        if (PIECES == 2)
+                            *reinterpret_cast<uint4 *>(to + OP) = make_uint4(lo[0], lo[1], lo[E / 2 - 2], lo[E / 2 - 1]);
+                    } else {
+                        *reinterpret_cast<uint2 *>(to) = make_uint2(hi[0], hi[1]);
+                        if (PIECES == 2) *reinterpret_cast<uint2 *>(to + OP) = make_uint2(lo[0], lo[1]);
+                    }
                 }
+                }
+                __syncwarp();
+                const float back = sh.back[t][row];
                 tqp::fence_proxy_async();
                 tqp::tc_fence_before(); // the last segment's reads of S and O
                 tqp::mbar_arrive(&sh.q_ready[t]);
 
                 for (int j = 0; j < mine; j++) {
-                    const int pos0 = (w.tile + j) * kPos, cs = (tick + j) % kConsts;
+                    const int cs = (tick + j) % kConsts;
+                    const int seen = lim - (tile0 + j) * kPos; // columns below it are visible
+                    const bool whole = __all_sync(0xffffffffu, seen >= kPos);
                     wait_slot(&sh.s_full[t], s_phase & 1, &sh.late, p.c.status);
                     s_phase++;
                     tqp::tc_fence_after();
-                    const int seen = lim - pos0; // columns below it are visible
-                    const bool whole = __all_sync(0xffffffffu, seen >= kPos);
+                    uint32_t v[4][32]; // the row of S
+#pragma unroll
+                    for (int c = 0; c < 4; c++) tmem_ld32(s_at + 32 * c, v[c]);
+                    tqp::tmem_wait_ld();
+                    if (!whole) { // what the row does not see
+#pragma unroll
+                        for (int c = 0; c < 4; c++)
+#pragma unroll
+                            for (int u = 0; u < 32; u++)
+                                if (32 * c + u >= seen) v[c][u] = 0xff800000u;
+                    }
                     // ---- M ----
                     float top = -INFINITY;
-#pragma unroll 1
-                    for (int c = 0; c < 4; c++) {
-                        uint32_t v[32];
-                        tmem_ld32(s_at + 32 * c, v);
-                        tqp::tmem_wait_ld();
 #pragma unroll
-                        for (int b = 0; b < 2; b++) {
-                            float mx = -INFINITY;
+                    for (int b = 0; b < kBlocks; b++) {
+                        const uint32_t *s = &v[b >> 1][16 * (b & 1)];
+                        float mx = __uint_as_float(s[0]);
 #pragma unroll
-                            for (int u = 0; u < 16; u++) {
-                                float s = __uint_as_float(v[16 * b + u]);
-                                if (!whole) s = 32 * c + 16 * b + u < seen ? s : -INFINITY;
-                                mx = fmaxf(mx, s);
-                            }
-                            top = fmaxf(top, fmaf(mx, sh.f[cs][2 * c + b] * back, sh.lv[cs][2 * c + b]));
-                        }
+                        for (int u = 1; u < 15; u += 2) mx = max3(mx, __uint_as_float(s[u]), __uint_as_float(s[u + 1]));
+                        mx = fmaxf(mx, __uint_as_float(s[15]));
+                        top = fmaxf(top, fmaf(mx, sh.f[cs][b] * back, sh.lv[cs][b]));
                     }
-                    float alpha = 1.f;
-                    if (top > M + kSlack || (M == -INFINITY && top > M)) {
-                        alpha = ex2(M - top);
+                    if (top > M + kSlack) {
+                        const float alpha = ex2(M - top);
                         M = top;
                         L *= alpha;
+                        top = alpha;
+                    } else {
+                        top = 1.f;
                     }
-                    if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+                    if (j > 0 && __any_sync(0xffffffffu, top != 1.f)) {
                         // S of this tile is complete, so O += P V of the last one is (issued before it)
 #pragma unroll 1
-                        for (int c = 0; c < HDP / 32; c++) {
-                            uint32_t v[32];
-                            tmem_ld32(o_at + 32 * c, v);
+                        for (int c = 0; c < HDP / 16; c++) {
+                            uint32_t o[16];
+                            tqp::tmem_ld16(o_at + 16 * c, o);
                             tqp::tmem_wait_ld();
 #pragma unroll
-                            for (int u = 0; u < 32; u++) v[u] = __float_as_uint(__uint_as_float(v[u]) * alpha);
-                            tmem_st32(o_at + 32 * c, v);
+                            for (int u = 0; u < 16; u++) o[u] = __float_as_uint(__uint_as_float(o[u]) * top);
+                            tmem_st16(o_at + 16 * c, o);
                         }
                     }
-                    const float use = M == -INFINITY ? 0.f : M - kUnit;
                     // ---- P over S ----
-#pragma unroll 1
+                    const float use = M == -INFINITY ? 0.f : M - kUnit;
+#pragma unroll
                     for (int c = 0; c < 4; c++) {
-                        uint32_t v[32], hi[16], lo[16];
-                        tmem_ld32(s_at + 32 * c, v);
-                        tqp::tmem_wait_ld();
+                        uint32_t hi[16], lo[16];
 #pragma unroll
                         for (int b = 0; b < 2; b++) {
                             const float fb = sh.f[cs][2 * c + b] * back, ob = sh.lv[cs][2 * c + b] - use;
                             float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
                             for (int u = 0; u < 16; u += 2) {
-                                const float2 s = make_float2(__uint_as_float(v[16 * b + u]), __uint_as_float(v[16 * b + u + 1]));
+                                const float2 s = make_float2(__uint_as_float(v[c][16 * b + u]), __uint_as_float(v[c][16 * b + u + 1]));
                                 const float2 e = __ffma2_rn(s, make_float2(fb, fb), make_float2(ob, ob));
-                                float2 y = make_float2(ex2(e.x), ex2(e.y));
-                                if (!whole) { // 0 whatever the block's scales are
-                                    y.x = 32 * c + 16 * b + u < seen ? y.x : 0.f;
-                                    y.y = 32 * c + 16 * b + u + 1 < seen ? y.y : 0.f;
-                                }
+                                const float2 y = make_float2(ex2(e.x), ex2(e.y));
                                 sum = __fadd2_rn(sum, y);
                                 const unsigned h = pack2(y.x, y.y);
                                 hi[8 * b + u / 2] = h;
@@ -482,6 +546,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const __grid_con
                             tmem_st16(s_at + 32 * c + 16, lo);
                         }
                     }
+                    // a scale that is not a number spoils the rows that see its block
+                    for (unsigned bad = sh.poison[cs]; bad; bad &= bad - 1)
+                        if (seen > (__ffs(bad) - 1) * TQ_KV_BLOCK) L = __int_as_float(0x7fc00000);
                     tmem_wait_st();
                     tqp::tc_fence_before();
                     tqp::mbar_arrive(&sh.p_ready[t]);
@@ -490,157 +557,139 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const __grid_con
                 o_phase++;
                 tqp::tc_fence_after();
             }
-            // ---- out, or this part of it ----
-            const bool all = w.from >= x0 && w.from + w.tiles <= x1;
-            if (all) {
-                const float inv = L == 0.f ? 0.f : 1.f / L;
-                T *o = static_cast<T *>(p.a.out) + (size_t)(w.s.start + tok) * p.a.out_stride + (size_t)hq * p.c.hd;
-                if (mine > 0)
+            // ---- out, or this part of it: some columns at a time through this warp's own rows of Q's memory
+            // (other warps may be loading theirs for the next segment) ----
+            constexpr int RB = PIECES * OP / kRows < 256 ? PIECES * OP / kRows : 256; // bytes of a row there
+            unsigned char *stage = Qs + t * PIECES * OP + (warp & 3) * (32 * 128);
+            auto staged = [&](int sr, int c) { // 16-byte chunk c of row sr of the warp
+                return reinterpret_cast<uint4 *>(stage + (c >> 3) * (kRows * 128) + sr * 128 + (((c & 7) ^ (sr & 7)) << 4));
+            };
+            auto spread = [&](auto one, float factor, auto &&at) { // one: the element type; at(row of the warp): its address
+                using X = decltype(one);
+                constexpr int E = 16 / sizeof(X), COLS = RB / (int)sizeof(X) < HDP ? RB / (int)sizeof(X) : HDP;
+                constexpr int LANES = COLS / E, ROWS = 32 / LANES;
 #pragma unroll 1
-                    for (int c = 0; c < HDP / 32; c++) {
-                        uint32_t v[32];
-                        tmem_ld32(o_at + 32 * c, v);
+                for (int h = 0; h < HDP; h += COLS) {
+                    __syncwarp();
+#pragma unroll 2
+                    for (int c = 0; c < COLS; c += 16) {
+                        uint32_t o[16];
+                        tqp::tmem_ld16(o_at + h + c, o);
                         tqp::tmem_wait_ld();
-                        if (live)
 #pragma unroll
-                            for (int u = 0; u < 32; u += 8)
-                                if (32 * c + u < p.c.hd) {
-                                    float y[8];
+                        for (int u = 0; u < 16; u += E) {
+                            __align__(16) X e[E];
 #pragma unroll
-                                    for (int e = 0; e < 8; e++) y[e] = __uint_as_float(v[u + e]) * inv;
-                                    store8(o + 32 * c + u, p.vec, y);
-                                }
+                            for (int k = 0; k < E; k += 2)
+                                Elem<X>::put2(e + k, __uint_as_float(o[u + k]) * factor, __uint_as_float(o[u + k + 1]) * factor,
+                                              true, true);
+                            *staged(lane, (c + u) / E) = *reinterpret_cast<const uint4 *>(e);
+                        }
                     }
+                    __syncwarp();
+                    const int c = lane % LANES;
+#pragma unroll 4
+                    for (int i = 0; i < 32 / ROWS; i++) {
+                        const int sr = i * ROWS + lane / LANES;
+                        at(sr, h + c * E, *staged(sr, c), __shfl_sync(0xffffffffu, o_at_row, sr));
+                    }
+                }
+                __syncwarp();
+            };
+            if (part_at < 0) {
+                if (mine > 0)
+                    spread(T(0.f), L == 0.f ? 0.f : 1.f / L, [&](int, int d, const uint4 &x, long long to) {
+                        if (to < 0 || d >= p.c.hd) return;
+                        T *o = static_cast<T *>(p.a.out) + to + d;
+                        if (p.vec) {
+                            *reinterpret_cast<uint4 *>(o) = x;
+                        } else {
+                            const T *e = reinterpret_cast<const T *>(&x);
+#pragma unroll
+                            for (int u = 0; u < 16 / (int)sizeof(T); u++) o[u] = e[u];
+                        }
+                    });
             } else {
                 float *part = reinterpret_cast<float *>(static_cast<char *>(p.a.workspace) + kKvHead) +
-                              ((size_t)blockIdx.x * 2 + (w.from >= x0 ? 1 : 0)) * partial_floats(HDP);
-                const int pr = t * kRows + row;
+                              ((size_t)blockIdx.x * 2 + part_at) * partial_floats(HDP);
                 if (mine > 0)
-#pragma unroll 1
-                    for (int c = 0; c < HDP / 32; c++) {
-                        uint32_t v[32];
-                        tmem_ld32(o_at + 32 * c, v);
-                        tqp::tmem_wait_ld();
-#pragma unroll
-                        for (int u = 0; u < 32; u += 4)
-                            *reinterpret_cast<uint4 *>(part + (size_t)pr * HDP + 32 * c + u) =
-                                make_uint4(v[u], v[u + 1], v[u + 2], v[u + 3]);
-                    }
-                part[kBlockRows * HDP + pr] = mine > 0 ? M : __int_as_float(0x7f800001); // a NaN: no part here
+                    spread(0.f, 1.f, [&](int sr, int d, const uint4 &x, long long) {
+                        *reinterpret_cast<uint4 *>(part + (size_t)(t * kRows + (warp & 3) * 32 + sr) * HDP + d) = x;
+                    });
+                const int pr = t * kRows + row;
+                part[kBlockRows * HDP + pr] = mine > 0 ? M : __int_as_float(0x7fc00000); // NaN: no part here
                 part[kBlockRows * HDP + kBlockRows + pr] = L;
             }
-            x += cnt;
             tick += cnt;
-            if (x < x1) next_segment(p, w);
         }
     } else if (warp < kMmaWarp) {
         // ================= codes -> float16 operands =================
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(conv_regs(PIECES)));
         const int ct = tid - 32 * kSoftWarps;
         constexpr int U = kPos * HDP / 16 / kConvThreads; // 16-byte words per thread and tile
         constexpr int PER_ROW = HDP / 16;
-        // the segment and tile that is loaded (ahead of what is converted)
-        Where ld = w;
-        long long lx = x0;
-        int lt = w.tile;
-        int id = -1; // lanes 0..7: the page of block `lane` of the tile being loaded
-        float2 sc = make_float2(0.f, 0.f), sc_keys;
-        uint4 rk[U], rv[U];
-        const float mag = fabsf(p.scale2);
-        auto fetch = [&]() {
-            id = -1;
-            sc = make_float2(-1.f, 0.f);
-            if (lx >= x1 || lane >= kBlocks) return;
-            const int pos = lt * kPos + lane * TQ_KV_BLOCK;
-            const int rows = ld.s.nq * group;
-            if (pos < sees(ld.s, min(rows, (ld.rb + 1) * kBlockRows) - 1, group)) {
-                id = p.a.table[(size_t)ld.i * p.a.table_stride + (pos >> p.c.page_shift)];
-                if (id < 0 || id >= p.c.n_pages) {
-                    id = -1;
-                    atomicOr(p.c.status, TQ_KV_STATUS_PAGE);
-                } else {
-                    sc = __ldg(p.c.scale + (size_t)id * p.c.n_kv + ld.head);
-                }
-            }
-        };
-        // word u of the thread: of block blk(u); keys: its row and chunk, values: its dimension
-        auto load = [&](const int8_t *from, uint4 (&r)[U], bool values) {
-#pragma unroll
-            for (int u = 0; u < U; u++) {
-                const int word = ct + u * kConvThreads, blk = word / HDP, in = word - blk * HDP; // HDP words a block
-                const int page = __shfl_sync(0xffffffffu, id, blk);
-                const float c = __shfl_sync(0xffffffffu, sc.y, blk);
-                r[u] = make_uint4(0, 0, 0, 0);
-                if (page >= 0 && !(values && c == 0.f)) {
-                    const int b = ((lt * kPos + blk * TQ_KV_BLOCK) & (p.c.page - 1)) >> 4;
-                    r[u] = __ldg(reinterpret_cast<const uint4 *>(from + kv_block_offset(p.c, page, ld.head, b)) + in);
-                }
-            }
-        };
+        static_assert(kPos * HDP / 16 == HDP * kBlocks, "a block is HDP words of 16 bytes");
         auto expand = [&](const uint4 &r, uint4 &lo, uint4 &hi) {
             cvt4(r.x, lo.x, lo.y);
             cvt4(r.y, lo.z, lo.w);
             cvt4(r.z, hi.x, hi.y);
             cvt4(r.w, hi.z, hi.w);
         };
-        auto step = [&]() { // to the next tile to be loaded
-            lx++;
-            lt++;
-            if (lx < x1 && lt == ld.tiles) {
-                next_segment(p, ld);
-                lt = 0;
-            }
+        // a staged word, or zeros for a block that is not there
+        auto word_of = [&](int side, int word, unsigned there) {
+            const uint4 w = *reinterpret_cast<const uint4 *>(Cs + side * CODES + word * 16);
+            return there >> (word / HDP) & 1 ? w : make_uint4(0, 0, 0, 0);
         };
-        static_assert(kPos * HDP / 16 == HDP * kBlocks, "a block is HDP words of 16 bytes");
-        fetch();
-        load(p.c.k, rk, false);
         unsigned k = 0;
-        const unsigned count = (unsigned)(x1 - x0);
-        for (k = 0; k < count; k++) {
-            const unsigned s = k % ST, round = k / ST;
-            sc_keys = sc;
-            load(p.c.v, rv, true);
-            // ---- keys of tile k ----
-            if (round > 0) wait_slot(&sh.k_empty[s], (round - 1) & 1, &sh.late, p.c.status);
-#pragma unroll
-            for (int u = 0; u < U; u++) {
-                const int word = ct + u * kConvThreads, r = word / PER_ROW, c = word - r * PER_ROW;
-                // where the cache keeps chunk c of the row (tq_kv.h): here the word is chunk c as stored
-                const int chunk = HDP >= 128 ? c ^ ((r & 1) << 2) : c; // 16 dimensions
-                uint4 a, b;
-                expand(rk[u], a, b);
-                unsigned char *to = Ks + s * OP + (chunk >> 2) * (kPos * 128);
-                const int c0 = 2 * (chunk & 3), h = HDP >= 128 ? chunk >> 2 & 1 : 0; // two halves in turn: distinct banks
-                *reinterpret_cast<uint4 *>(to + chunk_at(r, c0 + h)) = h ? b : a;
-                *reinterpret_cast<uint4 *>(to + chunk_at(r, c0 + 1 - h)) = h ? a : b;
+        for (unsigned n = 0;; n++) {
+            const int cnt = next_seg(n).cnt;
+            __syncwarp();
+            if (lane == 0) tqp::mbar_arrive(&sh.seg_empty[n % kSegs]);
+            if (cnt == 0) break;
+            for (const unsigned end = k + cnt; k < end; k++) {
+                const unsigned s = k % ST, round = k / ST;
+                // ---- keys ----
+                wait_slot(&sh.code_full[0], k & 1, &sh.late, p.c.status);
+                if (round > 0) wait_slot(&sh.k_empty[s], (round - 1) & 1, &sh.late, p.c.status);
+                unsigned there = sh.live[0];
+#pragma unroll 4
+                for (int u = 0; u < U; u++) {
+                    const int word = ct + u * kConvThreads, r = word / PER_ROW, c = word - r * PER_ROW;
+                    // the word is stored at c: the 16 dimensions of chunk c ^ .. (tq_kv.h)
+                    const int chunk = HDP >= 128 ? c ^ ((r & 1) << 2) : c;
+                    uint4 a, b;
+                    expand(word_of(0, word, there), a, b);
+                    unsigned char *to = Ks + s * OP + (chunk >> 2) * (kPos * 128);
+                    const int c0 = 2 * (chunk & 3), h = HDP >= 128 ? chunk >> 2 & 1 : 0; // halves in turn: distinct banks
+                    *reinterpret_cast<uint4 *>(to + chunk_at(r, c0 + h)) = h ? b : a;
+                    *reinterpret_cast<uint4 *>(to + chunk_at(r, c0 + 1 - h)) = h ? a : b;
+                }
+                tqp::fence_proxy_async();
+                tqp::mbar_arrive(&sh.k_full[s]);
+                __syncwarp();
+                if (lane == 0) tqp::mbar_arrive(&sh.code_empty[0]);
+                // ---- values ----
+                wait_slot(&sh.code_full[1], k & 1, &sh.late, p.c.status);
+                if (round > 0) wait_slot(&sh.v_empty[s], (round - 1) & 1, &sh.late, p.c.status);
+                there = sh.live[1];
+#pragma unroll 4
+                for (int u = 0; u < U; u++) {
+                    const int word = ct + u * kConvThreads, blk = word / HDP, d = word - blk * HDP;
+                    uint4 a, b;
+                    expand(word_of(1, word, there), a, b);
+                    unsigned char *to = Vs + s * OP + (blk >> 2) * (HDP * 128);
+                    *reinterpret_cast<uint4 *>(to + chunk_at(d, 2 * (blk & 3))) = a;
+                    *reinterpret_cast<uint4 *>(to + chunk_at(d, 2 * (blk & 3) + 1)) = b;
+                }
+                tqp::fence_proxy_async();
+                tqp::mbar_arrive(&sh.v_full[s]);
+                __syncwarp();
+                if (lane == 0) tqp::mbar_arrive(&sh.code_empty[1]);
             }
-            if (ct < kBlocks) { // the scales of the tile's blocks; x < 0: a block that is not there
-                const bool there = sc_keys.x >= 0.f || sc_keys.x != sc_keys.x;
-                const bool plain = sc_keys.y > 0.f;
-                sh.f[k % kConsts][ct] = there ? sc_keys.x * mag : 0.f;
-                sh.lv[k % kConsts][ct] = !there ? -INFINITY : plain ? log2f(sc_keys.y) : sc_keys.y == 0.f ? 0.f : sc_keys.y;
-                sh.rv[k % kConsts][ct] = !there ? 0.f : plain ? 1.f / sc_keys.y : 1.f;
-            }
-            tqp::fence_proxy_async();
-            tqp::mbar_arrive(&sh.k_full[s]);
-            step();
-            fetch();
-            load(p.c.k, rk, false);
-            // ---- values of tile k ----
-            if (round > 0) wait_slot(&sh.v_empty[s], (round - 1) & 1, &sh.late, p.c.status);
-#pragma unroll
-            for (int u = 0; u < U; u++) {
-                const int word = ct + u * kConvThreads, blk = word / HDP, d = word - blk * HDP;
-                uint4 a, b;
-                expand(rv[u], a, b);
-                unsigned char *to = Vs + s * OP + (blk >> 2) * (HDP * 128);
-                *reinterpret_cast<uint4 *>(to + chunk_at(d, 2 * (blk & 3))) = a;
-                *reinterpret_cast<uint4 *>(to + chunk_at(d, 2 * (blk & 3) + 1)) = b;
-            }
-            tqp::fence_proxy_async();
-            tqp::mbar_arrive(&sh.v_full[s]);
         }
-    } else {
+    } else if (warp == kMmaWarp) {
         // ================= MMA issue: one thread =================
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(mma_regs(PIECES)));
         if (lane == 0) {
             unsigned tick = 0, q_phase[2] = {0, 0}, p_phase[2] = {0, 0};
             const uint32_t q0 = tqp::smem_u32(Qs), k0 = tqp::smem_u32(Ks), v0 = tqp::smem_u32(Vs);
@@ -662,18 +711,20 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const __grid_con
                 for (int pc = 0; pc < PIECES; pc++)
 #pragma unroll
                     for (int ks = 0; ks < kPos / 16; ks++) {
-                        const uint32_t a = PIECES == 1 ? s_col(t) + 8 * ks : s_col(t) + 32 * (ks >> 1) + 16 * pc + 8 * (ks & 1);
+                        const uint32_t a =
+                            PIECES == 1 ? s_col(t) + 8 * ks : s_col(t) + 32 * (ks >> 1) + 16 * pc + 8 * (ks & 1);
                         mma_ts(o_col(t), a, desc(vb + (ks >> 2) * (HDP * 128) + (ks & 3) * 32), idesc_f16(HDP),
                                !first || pc > 0 || ks > 0);
                     }
             };
-            while (x < x1) {
-                const int cnt = (int)min((long long)(w.tiles - w.tile), x1 - x);
-                int mine[2];
-#pragma unroll
-                for (int t = 0; t < 2; t++) mine[t] = min(cnt, max(0, tiles_of(w, t, group) - w.tile));
+            for (unsigned sn = 0;; sn++) {
+                const Seg &g = next_seg(sn);
+                const int cnt = g.cnt, mine[2] = {g.mine[0], g.mine[1]};
+                tqp::mbar_arrive(&sh.seg_empty[sn % kSegs]);
+                if (cnt == 0) break;
                 for (int j = -1; j < cnt; j++) {
                     const unsigned n = tick + j;
+#pragma unroll
                     for (int t = 0; t < 2; t++) {
                         // every tile's operands are waited for once, whether a row tile uses them or not
                         if (j >= 0 && t == 0) wait_slot(&sh.v_full[n % ST], (n / ST) & 1, &sh.late, p.c.status);
@@ -694,11 +745,106 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const __grid_con
                         if (j + 1 < cnt && t == 1) tqp::umma_commit(&sh.k_empty[(n + 1) % ST]);
                     }
                 }
-                x += cnt;
                 tick += cnt;
-                if (x < x1) next_segment(p, w);
             }
         }
+    } else if (warp == kMmaWarp + 1) {
+        // ================= loader: segments, pages, codes =================
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(mma_regs(PIECES)));
+        const TqSplit split(total, G);
+        const long long x0 = split.start(blockIdx.x), x1 = split.start(blockIdx.x + 1);
+        const float mag = fabsf(p.scale2);
+        // Lanes 0..7 take a block of the tile each. A tile passes through three
+        // stages: its page is asked for, then its scales, then its codes; the
+        // first runs two tiles ahead of the last, across segments.
+        Where w = find(p, sums, x0);
+        __syncwarp(); // the sums are read: codes go over them
+        long long x = x0; // of the first stage
+        int left = 0, visible = 0;
+        unsigned n = 0;
+        const int *table = nullptr;
+        auto open = [&](bool more) { // hands the segment at w, or the end, to the other roles
+            left = more ? (int)min((long long)(w.tiles - w.tile), x1 - x) : 0;
+            if (n >= kSegs) wait_slot(&sh.seg_empty[n % kSegs], (n / kSegs - 1) & 1, &sh.late, p.c.status);
+            if (lane == 0) {
+                Seg &g = sh.seg[n % kSegs];
+                g.cnt = left;
+                if (more) {
+                    g.start = w.s.start, g.nq = w.s.nq, g.len = w.s.len;
+                    g.head = w.head, g.row0 = w.rb * kBlockRows;
+                    g.tile = w.tile;
+                    for (int t = 0; t < 2; t++) g.mine[t] = min(left, max(0, tiles_of(w, t, group) - w.tile));
+                    g.part = w.from >= x0 && w.from + w.tiles <= x1 ? -1 : w.from >= x0 ? 1 : 0;
+                }
+                tqp::mbar_arrive(&sh.seg_full[n % kSegs]);
+            }
+            n++;
+            visible = more ? sees(w.s, min(w.s.nq * group, (w.rb + 1) * kBlockRows) - 1, group) : 0;
+            table = p.a.table + (size_t)w.i * p.a.table_stride;
+        };
+        struct Block {
+            int id, head, in;  // page, KV head, block of the page; id < 0: not there
+            bool wanted;
+        };
+        auto ask_page = [&]() { // first stage: the next tile
+            Block b{-1, 0, 0, false};
+            if (x >= x1) return b;
+            const int pos = w.tile * kPos + lane * TQ_KV_BLOCK;
+            b.head = w.head;
+            b.in = (pos & (p.c.page - 1)) >> 4;
+            b.wanted = lane < kBlocks && pos < visible;
+            if (b.wanted) b.id = __ldg(table + (pos >> p.c.page_shift));
+            x++, w.tile++;
+            if (--left == 0) {
+                if (x < x1) next_segment(p, w);
+                open(x < x1);
+            }
+            return b;
+        };
+        auto ask_scales = [&](Block &b) { // second stage
+            if (b.wanted && (b.id < 0 || b.id >= p.c.n_pages)) {
+                atomicOr(p.c.status, TQ_KV_STATUS_PAGE);
+                b.id = -1;
+            }
+            return b.id >= 0 ? __ldg(p.c.scale + (size_t)b.id * p.c.n_kv + b.head) : make_float2(0.f, 0.f);
+        };
+        open(true);
+        Block b0 = ask_page(), b1 = ask_page();
+        float2 sc = ask_scales(b0);
+        const unsigned count = (unsigned)(x1 - x0);
+        for (unsigned k = 0; k < count; k++) {
+            const Block b2 = ask_page();
+            const float2 sc1 = ask_scales(b1);
+            const bool there = b0.id >= 0, some = there && sc.y != 0.f;
+            const size_t at = there ? kv_block_offset(p.c, b0.id, b0.head, b0.in) : 0;
+            const unsigned keys = __ballot_sync(0xffffffffu, there), values = __ballot_sync(0xffffffffu, some);
+            const unsigned nan = __ballot_sync(0xffffffffu, there && (sc.x != sc.x || sc.y != sc.y));
+            // ---- keys, and the scales ----
+            if (k > 0) wait_slot(&sh.code_empty[0], (k - 1) & 1, &sh.late, p.c.status);
+            if (lane < kBlocks) {
+                const bool use = there && !(nan >> lane & 1), plain = use && sc.y > 0.f;
+                sh.f[k % kConsts][lane] = use ? fmaxf(sc.x * mag, kLeast) : kLeast;
+                sh.lv[k % kConsts][lane] = !use ? -INFINITY : plain ? log2f(sc.y) : 0.f;
+                sh.rv[k % kConsts][lane] = !use ? 0.f : plain ? 1.f / sc.y : 1.f;
+            }
+            if (lane == 0) sh.live[0] = keys, sh.poison[k % kConsts] = nan;
+            __syncwarp();
+            if (lane == 0) tqp::mbar_arrive_expect_tx(&sh.code_full[0], __popc(keys) * TQ_KV_BLOCK * HDP);
+            __syncwarp();
+            if (there) tqp::bulk_load(Cs + lane * TQ_KV_BLOCK * HDP, p.c.k + at, TQ_KV_BLOCK * HDP, &sh.code_full[0]);
+            // ---- values ----
+            if (k > 0) wait_slot(&sh.code_empty[1], (k - 1) & 1, &sh.late, p.c.status);
+            if (lane == 0) {
+                sh.live[1] = values;
+                tqp::mbar_arrive_expect_tx(&sh.code_full[1], __popc(values) * TQ_KV_BLOCK * HDP);
+            }
+            __syncwarp();
+            if (some)
+                tqp::bulk_load(Cs + CODES + lane * TQ_KV_BLOCK * HDP, p.c.v + at, TQ_KV_BLOCK * HDP, &sh.code_full[1]);
+            b0 = b1, b1 = b2, sc = sc1;
+        }
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(mma_regs(PIECES)));
     }
     __syncwarp();
     tqp::tc_fence_before();
