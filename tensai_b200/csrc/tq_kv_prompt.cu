@@ -21,9 +21,10 @@
 // the value scale rides in the exponent at no cost, and P stays below 2^14. A
 // block of value scale 0 counts with c = 1 and zero codes.
 //
-// Work: (sequence, KV head, row block) segments x position tiles, laid end to end
-// and cut evenly over one CTA per SM. A cut segment's parts go to the workspace;
-// the second kernel joins them in order (a fixed order: the same bits each time).
+// Work: (sequence, KV head, row block) segments laid end to end, each as long as
+// its position tiles and kSegCost units before them (its queries come in and its
+// outputs go out), and cut evenly over one CTA per SM. A cut segment's parts go to
+// the workspace; the second kernel joins them in order (the same bits each time).
 //
 // Bound by the exponentials (16 a cycle and SM) and the tensor cores alike: 128
 // positions of 128 rows take about 1024 cycles of each at head size 128.
@@ -43,15 +44,10 @@ constexpr int kBlocks = kPos / TQ_KV_BLOCK;
 constexpr int kSoftWarps = 8, kConvWarps = 4;
 constexpr int kConvThreads = 32 * kConvWarps;
 constexpr int kMmaWarp = kSoftWarps + kConvWarps; // one thread of it issues; the next warp loads
-constexpr int kThreads = 32 * (kMmaWarp + 4);      // four warpgroups, for the split of the registers:
-// softmax (a row of S stays in registers), widening, the rest.
-constexpr int soft_regs(int pieces) { return pieces == 1 ? 192 : 176; }
-constexpr int conv_regs(int pieces) { return pieces == 1 ? 64 : 72; }
-constexpr int mma_regs(int pieces) { return pieces == 1 ? 64 : 88; }
-static_assert(2 * soft_regs(1) + conv_regs(1) + mma_regs(1) <= 4 * 128, "no more than the launch's registers");
-static_assert(2 * soft_regs(2) + conv_regs(2) + mma_regs(2) <= 4 * 128, "no more than the launch's registers");
+constexpr int kThreads = 32 * (kMmaWarp + 2);
 constexpr int kConsts = 4;      // position tiles whose scales are kept
-constexpr int kMinTiles = 2;    // position tiles per CTA below which fewer CTAs work
+constexpr int kSegCost = 3;     // what a segment costs besides its position tiles, in position tiles
+constexpr int kMinUnits = 5;    // units per CTA below which fewer CTAs work
 constexpr float kSlack = 4.f;   // log2 by which w may exceed M
 constexpr float kUnit = 10.f;   // log2 of P at w = M
 constexpr float kLeast = 1e-30f; // least score factor of a block: -inf times it stays -inf
@@ -83,20 +79,22 @@ __device__ __forceinline__ Blocks blocks_of(const Seq &s, int group) {
     b.first = s.nq > s.len ? 0u : (unsigned)(s.len - s.nq + 1);
     return b;
 }
-// The position tiles of one head, by a whole warp.
-__device__ __forceinline__ long long head_tiles(const Blocks &b, int group) {
+// The units of one head, by a whole warp.
+__device__ __forceinline__ long long head_units(const Blocks &b, int group) {
     long long t = 0;
-    for (int rb = threadIdx.x & 31; rb < b.nrb; rb += 32) t += b.tiles(rb, group);
+    for (int rb = threadIdx.x & 31; rb < b.nrb; rb += 32) t += b.tiles(rb, group) + kSegCost;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
     return t;
 }
 
-struct Where { // a segment and a position tile of it
-    int i, head, rb, tile, tiles;
+struct Where { // a segment
+    int i, head, rb, tiles;
     Seq s;
     Blocks b;
-    long long from; // the segment's first position tile in the list
+    long long from; // where its position tiles begin in the list (its own cost lies before)
+    // the position tiles [a, z) of it that lie in the units [x0, x1) of the list
+    __device__ __forceinline__ int first(long long x0) const { return (int)min((long long)tiles, max(0ll, x0 - from)); }
 };
 
 __device__ __forceinline__ Seq prompt_seq(const Params &p, int i) {
@@ -105,7 +103,7 @@ __device__ __forceinline__ Seq prompt_seq(const Params &p, int i) {
     return s;
 }
 
-// sums[e] = position tiles of the sequences before entry e, for all threads of a block; the total.
+// sums[e] = units of the sequences before entry e, for all threads of a block; the total.
 template <int NT> __device__ __forceinline__ long long list_sums(const Params &p, long long *sums) {
     constexpr int NW = NT / 32, PER = (kKvSums + NT - 1) / NT;
     __shared__ long long scan[NW];
@@ -119,12 +117,12 @@ template <int NT> __device__ __forceinline__ long long list_sums(const Params &p
         Seq s{0, 0, 0};
         if (i < n) s = prompt_seq(p, i);
         const Blocks b = blocks_of(s, p.group);
-        long long t = s.nq && b.nrb == 1 ? b.tiles(0, p.group) : 0;
+        long long t = s.nq && b.nrb == 1 ? b.tiles(0, p.group) + kSegCost : 0;
         for (unsigned many = __ballot_sync(0xffffffffu, s.nq && b.nrb > 1); many; many &= many - 1) {
             const int l = __ffs(many) - 1;
             const Blocks o = {__shfl_sync(0xffffffffu, b.nrb, l), __shfl_sync(0xffffffffu, b.last, l),
                               __shfl_sync(0xffffffffu, b.first, l)};
-            const long long all = head_tiles(o, p.group);
+            const long long all = head_units(o, p.group);
             if (lane == l) t = all;
         }
         if (t)
@@ -165,7 +163,7 @@ template <int NT> __device__ __forceinline__ long long list_sums(const Params &p
     return total;
 }
 
-// The segment that holds position tile x of the list; called by whole warps.
+// The segment that holds unit x of the list; called by whole warps.
 __device__ __forceinline__ Where find(const Params &p, const long long *sums, long long x) {
     const int lane = threadIdx.x & 31;
     const int entries = (p.a.n + (1 << p.shift_sums) - 1) >> p.shift_sums;
@@ -184,7 +182,7 @@ __device__ __forceinline__ Where find(const Params &p, const long long *sums, lo
         w.s = prompt_seq(p, w.i);
         if (w.s.nq == 0) continue;
         w.b = blocks_of(w.s, p.group);
-        const long long per = head_tiles(w.b, p.group);
+        const long long per = head_units(w.b, p.group);
         if (rest < per * p.c.n_kv) {
             for (; rest >= per; rest -= per) w.head++;
             break;
@@ -192,7 +190,7 @@ __device__ __forceinline__ Where find(const Params &p, const long long *sums, lo
         rest -= per * p.c.n_kv;
     }
     for (int r0 = 0;; r0 += 32) { // 32 row blocks at a time
-        const int mine = r0 + lane < w.b.nrb ? w.b.tiles(r0 + lane, p.group) : 0;
+        const int mine = r0 + lane < w.b.nrb ? w.b.tiles(r0 + lane, p.group) + kSegCost : 0;
         long long upto = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -203,19 +201,18 @@ __device__ __forceinline__ Where find(const Params &p, const long long *sums, lo
         if (beyond || r0 + 32 >= w.b.nrb) {
             const int l = beyond ? __ffs(beyond) - 1 : 31;
             w.rb = r0 + l;
-            w.tiles = __shfl_sync(0xffffffffu, mine, l);
-            w.tile = (int)(rest - (__shfl_sync(0xffffffffu, upto, l) - w.tiles));
+            const int units = __shfl_sync(0xffffffffu, mine, l);
+            w.tiles = units - kSegCost;
+            w.from = x - (rest - (__shfl_sync(0xffffffffu, upto, l) - units)) + kSegCost;
             break;
         }
         rest -= __shfl_sync(0xffffffffu, upto, 31);
     }
-    w.from = x - w.tile;
     return w;
 }
 
 __device__ __forceinline__ void next_segment(const Params &p, Where &w) {
-    w.from += w.tiles;
-    w.tile = 0;
+    w.from += w.tiles + kSegCost;
     if (++w.rb == w.b.nrb) {
         w.rb = 0;
         if (++w.head == p.c.n_kv) {
@@ -337,7 +334,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const __grid_con
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int group = p.group;
     const long long total = list_sums<kThreads>(p, sums);
-    const int G = (int)min((long long)gridDim.x, (total + kMinTiles - 1) / kMinTiles);
+    const int G = (int)min((long long)gridDim.x, (total + kMinUnits - 1) / kMinUnits);
     if ((int)blockIdx.x >= G) return; // none: G = 0
 
     if (tid == 0) {
@@ -380,7 +377,6 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const __grid_con
 
     if (warp < kSoftWarps) {
         // ================= softmax: thread = row of tile t =================
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(soft_regs(PIECES)));
         const int t = warp >> 2, row = (warp & 3) * 32 + lane;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t s_at = s_col(t) + lanes, o_at = o_col(t) + lanes;
@@ -401,65 +397,80 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const __grid_con
             const int lim = r < rows ? min(len, max(0, len - fresh + tok + 1)) : len;
             float M = -INFINITY, L = 0.f;
             if (mine > 0) {
-                // ---- Q, as float16 pieces: the warp's 32 rows, each by as many lanes as it has 16-byte words ----
+                // ---- Q, as float16 pieces: the warp's 32 rows, each by as many lanes as it has 16-byte words.
+                // The words come into the row's own memory (128 bytes for each 64 dimensions and piece)
+                // and are replaced there by the pieces.
                 constexpr int E = 16 / sizeof(T), LANES = HDP / E, ROWS = 32 / LANES;
                 unsigned char *qs = Qs + t * PIECES * OP;
-                const int d = (lane % LANES) * E;
-                constexpr int BATCH = 8; // words in flight
+                const int word = lane % LANES, d = word * E, sub = lane / LANES;
+                auto raw_at = [&](int qrow) {
+                    return reinterpret_cast<uint4 *>(qs + (word >> 3) * (kRows * 128) + chunk_at(qrow, word & 7));
+                };
+                constexpr int BATCH = 4; // rows a lane works on at once
+                if (p.vec) {
+#pragma unroll 4
+                    for (int i = 0; i < 32; i += ROWS) {
+                        const long long at = __shfl_sync(0xffffffffu, q_at, i + sub);
+                        const bool there = at >= 0 && d < p.c.hd;
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                                         tqp::smem_u32(raw_at((warp & 3) * 32 + i + sub))),
+                                     "l"(static_cast<const T *>(p.a.q) + (there ? at + d : 0)), "r"(there ? 16 : 0)
+                                     : "memory");
+                    }
+                } else {
 #pragma unroll 1
-                for (int i0 = 0; i0 < 32 / ROWS; i0 += BATCH) {
-                    uint4 word[BATCH];
-                    const T *from[BATCH];
+                    for (int i = 0; i < 32; i += ROWS) {
+                        const long long at = __shfl_sync(0xffffffffu, q_at, i + sub);
+                        const bool there = at >= 0 && d < p.c.hd;
+                        T *to = reinterpret_cast<T *>(raw_at((warp & 3) * 32 + i + sub));
+#pragma unroll 1
+                        for (int e = 0; e < E; e++) to[e] = there ? static_cast<const T *>(p.a.q)[at + d + e] : T(0.f);
+                    }
+                }
+                asm volatile("cp.async.wait_all;" ::: "memory");
+                __syncwarp();
+#pragma unroll 1
+                for (int i = 0; i < 32; i += ROWS * BATCH) {
+                    uint4 w[BATCH];
+                    float big[BATCH];
+#pragma unroll
+                    for (int u = 0; u < BATCH; u++) w[u] = *raw_at((warp & 3) * 32 + i + u * ROWS + sub);
 #pragma unroll
                     for (int u = 0; u < BATCH; u++) {
-                        const int sr = (i0 + u) * ROWS + lane / LANES;
-                        const long long at = __shfl_sync(0xffffffffu, q_at, sr & 31);
-                        from[u] = sr < 32 && at >= 0 && d < p.c.hd ? static_cast<const T *>(p.a.q) + at + d : nullptr;
-                    }
-                    if (p.vec) {
+                        big[u] = 0.f;
 #pragma unroll
-                        for (int u = 0; u < BATCH; u++)
-                            word[u] = from[u] ? __ldg(reinterpret_cast<const uint4 *>(from[u])) : make_uint4(0, 0, 0, 0);
-                    } else {
-#pragma unroll
-                        for (int u = 0; u < BATCH; u++)
-#pragma unroll
-                            for (int e = 0; e < E; e++) reinterpret_cast<T *>(&word[u])[e] = from[u] ? from[u][e] : T(0.f);
+                        for (int e = 0; e < E; e++)
+                            big[u] = fmaxf(big[u], fabsf(Elem<T>::get(reinterpret_cast<const T *>(&w[u]) + e)));
                     }
 #pragma unroll
-                for (int i = 0; i < BATCH; i++) {
-                    if (i0 + i >= 32 / ROWS) break;
-                    const int qrow = (warp & 3) * 32 + (i0 + i) * ROWS + lane / LANES;
-                    float y[E];
+                    for (int o = 1; o < LANES; o <<= 1) // all lanes of a row have read their word after this
 #pragma unroll
-                    for (int e = 0; e < E; e++) y[e] = Elem<T>::get(reinterpret_cast<const T *>(&word[i]) + e);
-                    float big = 0.f, was;
+                        for (int u = 0; u < BATCH; u++) big[u] = fmaxf(big[u], __shfl_xor_sync(0xffffffffu, big[u], o));
 #pragma unroll
-                    for (int u = 0; u < E; u++) big = fmaxf(big, fabsf(y[u]));
+                    for (int u = 0; u < BATCH; u++) {
+                        const int qrow = (warp & 3) * 32 + i + u * ROWS + sub;
+                        float was, unit = row_scale(big[u], &was);
+                        if (p.scale2 < 0.f) unit = -unit; // the block factors stay positive
+                        if (word == 0) sh.back[t][qrow] = was;
+                        unsigned hi[E / 2], lo[E / 2];
 #pragma unroll
-                    for (int o = 1; o < LANES; o <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
-                    float unit = row_scale(big, &was);
-                    if (p.scale2 < 0.f) unit = -unit; // the block factors stay positive
-                    if (lane % LANES == 0) sh.back[t][qrow] = was;
-                    unsigned hi[E / 2], lo[E / 2];
-#pragma unroll
-                    for (int u = 0; u < E / 2; u++) {
-                        const float a = y[2 * u] * unit, b = y[2 * u + 1] * unit;
-                        hi[u] = pack2(a, b);
-                        const float2 h = unpack2(hi[u]);
-                        lo[u] = pack2(a - h.x, b - h.y);
-                    }
-                    unsigned char *to = qs + (d >> 6) * (kRows * 128) + chunk_at(qrow, (d & 63) >> 3) + 2 * (d & 7);
-                    if (E == 8) {
-                        *reinterpret_cast<uint4 *>(to) = make_uint4(hi[0], hi[1], hi[E / 2 - 2], hi[E / 2 - 1]);
-                        if (PIECES == 2)
-                            *reinterpret_cast<uint4 *>(to + OP) = make_uint4(lo[0], lo[1], lo[E / 2 - 2], lo[E / 2 - 1]);
-                    } else {
-                        *reinterpret_cast<uint2 *>(to) = make_uint2(hi[0], hi[1]);
-                        if (PIECES == 2) *reinterpret_cast<uint2 *>(to + OP) = make_uint2(lo[0], lo[1]);
+                        for (int e = 0; e < E / 2; e++) {
+                            const float a = Elem<T>::get(reinterpret_cast<const T *>(&w[u]) + 2 * e) * unit;
+                            const float b = Elem<T>::get(reinterpret_cast<const T *>(&w[u]) + 2 * e + 1) * unit;
+                            hi[e] = pack2(a, b);
+                            const float2 h = unpack2(hi[e]);
+                            lo[e] = pack2(a - h.x, b - h.y);
+                        }
+                        unsigned char *to = qs + (d >> 6) * (kRows * 128) + chunk_at(qrow, (d & 63) >> 3) + 2 * (d & 7);
+                        if (E == 8) {
+                            *reinterpret_cast<uint4 *>(to) = make_uint4(hi[0], hi[1], hi[E / 2 - 2], hi[E / 2 - 1]);
+                        } else {
+                            *reinterpret_cast<uint2 *>(to) = make_uint2(hi[0], hi[1]);
+                            *reinterpret_cast<uint2 *>(to + OP) = make_uint2(lo[0], lo[1]);
+                        }
                     }
                 }
-                }
+                static_assert((sizeof(T) == 4) == (PIECES == 2), "a row's pieces take the room of its elements");
                 __syncwarp();
                 const float back = sh.back[t][row];
                 tqp::fence_proxy_async();
@@ -473,28 +484,49 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const __grid_con
                     wait_slot(&sh.s_full[t], s_phase & 1, &sh.late, p.c.status);
                     s_phase++;
                     tqp::tc_fence_after();
-                    uint32_t v[4][32]; // the row of S
+                    // S comes through 32 registers at a time, the next 32 on their way; the
+                    // loops are kept short: straight code of a whole row runs at the rate
+                    // at which instructions arrive.
+                    auto over = [&](auto &&use) {
+                        uint32_t v0[32], v1[32];
+                        tmem_ld32(s_at, v0);
+                        tqp::tmem_wait_ld();
+#pragma unroll 1
+                        for (int c = 0; c < 4; c += 2) {
+                            tmem_ld32(s_at + 32 * (c + 1), v1);
+                            use(c, v0);
+                            tqp::tmem_wait_ld();
+                            if (c == 0) tmem_ld32(s_at + 64, v0);
+                            use(c + 1, v1);
+                            tqp::tmem_wait_ld();
+                        }
+                    };
+                    if (!whole) { // what a row does not see
+#pragma unroll 1
+                        for (int c = 0; c < kPos; c += 16) {
+                            uint32_t v[16];
+                            tqp::tmem_ld16(s_at + c, v);
+                            tqp::tmem_wait_ld();
 #pragma unroll
-                    for (int c = 0; c < 4; c++) tmem_ld32(s_at + 32 * c, v[c]);
-                    tqp::tmem_wait_ld();
-                    if (!whole) { // what the row does not see
-#pragma unroll
-                        for (int c = 0; c < 4; c++)
-#pragma unroll
-                            for (int u = 0; u < 32; u++)
-                                if (32 * c + u >= seen) v[c][u] = 0xff800000u;
+                            for (int u = 0; u < 16; u++)
+                                if (c + u >= seen) v[u] = 0xff800000u; // -inf
+                            tmem_st16(s_at + c, v);
+                        }
+                        tmem_wait_st();
                     }
                     // ---- M ----
                     float top = -INFINITY;
+                    over([&](int c, const uint32_t (&v)[32]) {
 #pragma unroll
-                    for (int b = 0; b < kBlocks; b++) {
-                        const uint32_t *s = &v[b >> 1][16 * (b & 1)];
-                        float mx = __uint_as_float(s[0]);
+                        for (int b = 0; b < 2; b++) {
+                            float mx = __uint_as_float(v[16 * b]);
 #pragma unroll
-                        for (int u = 1; u < 15; u += 2) mx = max3(mx, __uint_as_float(s[u]), __uint_as_float(s[u + 1]));
-                        mx = fmaxf(mx, __uint_as_float(s[15]));
-                        top = fmaxf(top, fmaf(mx, sh.f[cs][b] * back, sh.lv[cs][b]));
-                    }
+                            for (int u = 1; u < 15; u += 2)
+                                mx = max3(mx, __uint_as_float(v[16 * b + u]), __uint_as_float(v[16 * b + u + 1]));
+                            mx = fmaxf(mx, __uint_as_float(v[16 * b + 15]));
+                            top = fmaxf(top, fmaf(mx, sh.f[cs][2 * c + b] * back, sh.lv[cs][2 * c + b]));
+                        }
+                    });
                     if (top > M + kSlack) {
                         const float alpha = ex2(M - top);
                         M = top;
@@ -515,10 +547,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const __grid_con
                             tmem_st16(o_at + 16 * c, o);
                         }
                     }
-                    // ---- P over S ----
+                    // ---- P over S: chunk c's 16 (or, in two pieces, 32) columns lie in columns already read ----
                     const float use = M == -INFINITY ? 0.f : M - kUnit;
-#pragma unroll
-                    for (int c = 0; c < 4; c++) {
+                    over([&](int c, const uint32_t (&v)[32]) {
                         uint32_t hi[16], lo[16];
 #pragma unroll
                         for (int b = 0; b < 2; b++) {
@@ -526,7 +557,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const __grid_con
                             float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
                             for (int u = 0; u < 16; u += 2) {
-                                const float2 s = make_float2(__uint_as_float(v[c][16 * b + u]), __uint_as_float(v[c][16 * b + u + 1]));
+                                const float2 s = make_float2(__uint_as_float(v[16 * b + u]), __uint_as_float(v[16 * b + u + 1]));
                                 const float2 e = __ffma2_rn(s, make_float2(fb, fb), make_float2(ob, ob));
                                 const float2 y = make_float2(ex2(e.x), ex2(e.y));
                                 sum = __fadd2_rn(sum, y);
@@ -545,7 +576,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const __grid_con
                             tmem_st16(s_at + 32 * c, hi);
                             tmem_st16(s_at + 32 * c + 16, lo);
                         }
-                    }
+                    });
                     // a scale that is not a number spoils the rows that see its block
                     for (unsigned bad = sh.poison[cs]; bad; bad &= bad - 1)
                         if (seen > (__ffs(bad) - 1) * TQ_KV_BLOCK) L = __int_as_float(0x7fc00000);
@@ -571,7 +602,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const __grid_con
 #pragma unroll 1
                 for (int h = 0; h < HDP; h += COLS) {
                     __syncwarp();
-#pragma unroll 2
+#pragma unroll 1
                     for (int c = 0; c < COLS; c += 16) {
                         uint32_t o[16];
                         tqp::tmem_ld16(o_at + h + c, o);
@@ -588,10 +619,21 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const __grid_con
                     }
                     __syncwarp();
                     const int c = lane % LANES;
-#pragma unroll 4
-                    for (int i = 0; i < 32 / ROWS; i++) {
-                        const int sr = i * ROWS + lane / LANES;
-                        at(sr, h + c * E, *staged(sr, c), __shfl_sync(0xffffffffu, o_at_row, sr));
+#pragma unroll 1
+                    for (int i = 0; i < 32; i += 4 * ROWS) {
+                        uint4 x[4];
+                        long long to[4];
+#pragma unroll
+                        for (int u = 0; u < 4; u++) {
+                            const int sr = (i + u * ROWS + lane / LANES) & 31;
+                            x[u] = *staged(sr, c);
+                            to[u] = __shfl_sync(0xffffffffu, o_at_row, sr);
+                        }
+#pragma unroll
+                        for (int u = 0; u < 4; u++) {
+                            const int sr = i + u * ROWS + lane / LANES;
+                            if (sr < 32) at(sr, h + c * E, x[u], to[u]);
+                        }
                     }
                 }
                 __syncwarp();
@@ -624,7 +666,6 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const __grid_con
         }
     } else if (warp < kMmaWarp) {
         // ================= codes -> float16 operands =================
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(conv_regs(PIECES)));
         const int ct = tid - 32 * kSoftWarps;
         constexpr int U = kPos * HDP / 16 / kConvThreads; // 16-byte words per thread and tile
         constexpr int PER_ROW = HDP / 16;
@@ -652,7 +693,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const __grid_con
                 wait_slot(&sh.code_full[0], k & 1, &sh.late, p.c.status);
                 if (round > 0) wait_slot(&sh.k_empty[s], (round - 1) & 1, &sh.late, p.c.status);
                 unsigned there = sh.live[0];
-#pragma unroll 4
+#pragma unroll 2
                 for (int u = 0; u < U; u++) {
                     const int word = ct + u * kConvThreads, r = word / PER_ROW, c = word - r * PER_ROW;
                     // the word is stored at c: the 16 dimensions of chunk c ^ .. (tq_kv.h)
@@ -672,7 +713,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const __grid_con
                 wait_slot(&sh.code_full[1], k & 1, &sh.late, p.c.status);
                 if (round > 0) wait_slot(&sh.v_empty[s], (round - 1) & 1, &sh.late, p.c.status);
                 there = sh.live[1];
-#pragma unroll 4
+#pragma unroll 2
                 for (int u = 0; u < U; u++) {
                     const int word = ct + u * kConvThreads, blk = word / HDP, d = word - blk * HDP;
                     uint4 a, b;
@@ -689,7 +730,6 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const __grid_con
         }
     } else if (warp == kMmaWarp) {
         // ================= MMA issue: one thread =================
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(mma_regs(PIECES)));
         if (lane == 0) {
             unsigned tick = 0, q_phase[2] = {0, 0}, p_phase[2] = {0, 0};
             const uint32_t q0 = tqp::smem_u32(Qs), k0 = tqp::smem_u32(Ks), v0 = tqp::smem_u32(Vs);
@@ -724,7 +764,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const __grid_con
                 if (cnt == 0) break;
                 for (int j = -1; j < cnt; j++) {
                     const unsigned n = tick + j;
-#pragma unroll
+#pragma unroll 1
                     for (int t = 0; t < 2; t++) {
                         // every tile's operands are waited for once, whether a row tile uses them or not
                         if (j >= 0 && t == 0) wait_slot(&sh.v_full[n % ST], (n / ST) & 1, &sh.late, p.c.status);
@@ -748,9 +788,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const __grid_con
                 tick += cnt;
             }
         }
-    } else if (warp == kMmaWarp + 1) {
+    } else {
         // ================= loader: segments, pages, codes =================
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(mma_regs(PIECES)));
         const TqSplit split(total, G);
         const long long x0 = split.start(blockIdx.x), x1 = split.start(blockIdx.x + 1);
         const float mag = fabsf(p.scale2);
@@ -759,45 +798,54 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const __grid_con
         // first runs two tiles ahead of the last, across segments.
         Where w = find(p, sums, x0);
         __syncwarp(); // the sums are read: codes go over them
-        long long x = x0; // of the first stage
-        int left = 0, visible = 0;
+        int tile = 0, left = 0, visible = 0; // of the first stage
         unsigned n = 0;
         const int *table = nullptr;
-        auto open = [&](bool more) { // hands the segment at w, or the end, to the other roles
-            left = more ? (int)min((long long)(w.tiles - w.tile), x1 - x) : 0;
+        // Hands the segment at w, or the next that has position tiles here, to the
+        // other roles; without one, the end.
+        auto open = [&]() {
+            for (;; next_segment(p, w)) {
+                left = 0;
+                if (w.i >= p.a.n || w.from - kSegCost >= x1) break;
+                tile = w.first(x0);
+                left = w.first(x1) - tile;
+                if (left > 0) break;
+            }
             if (n >= kSegs) wait_slot(&sh.seg_empty[n % kSegs], (n / kSegs - 1) & 1, &sh.late, p.c.status);
             if (lane == 0) {
                 Seg &g = sh.seg[n % kSegs];
                 g.cnt = left;
-                if (more) {
+                if (left > 0) {
                     g.start = w.s.start, g.nq = w.s.nq, g.len = w.s.len;
                     g.head = w.head, g.row0 = w.rb * kBlockRows;
-                    g.tile = w.tile;
-                    for (int t = 0; t < 2; t++) g.mine[t] = min(left, max(0, tiles_of(w, t, group) - w.tile));
-                    g.part = w.from >= x0 && w.from + w.tiles <= x1 ? -1 : w.from >= x0 ? 1 : 0;
+                    g.tile = tile;
+                    for (int t = 0; t < 2; t++) g.mine[t] = min(left, max(0, tiles_of(w, t, group) - tile));
+                    g.part = left == w.tiles ? -1 : tile == 0 ? 1 : 0;
                 }
                 tqp::mbar_arrive(&sh.seg_full[n % kSegs]);
             }
             n++;
-            visible = more ? sees(w.s, min(w.s.nq * group, (w.rb + 1) * kBlockRows) - 1, group) : 0;
+            if (left == 0) return;
+            visible = sees(w.s, min(w.s.nq * group, (w.rb + 1) * kBlockRows) - 1, group);
             table = p.a.table + (size_t)w.i * p.a.table_stride;
         };
         struct Block {
             int id, head, in;  // page, KV head, block of the page; id < 0: not there
-            bool wanted;
+            bool wanted, some; // some: there is such a tile
         };
         auto ask_page = [&]() { // first stage: the next tile
-            Block b{-1, 0, 0, false};
-            if (x >= x1) return b;
-            const int pos = w.tile * kPos + lane * TQ_KV_BLOCK;
+            Block b{-1, 0, 0, false, false};
+            if (left == 0) return b;
+            const int pos = tile * kPos + lane * TQ_KV_BLOCK;
             b.head = w.head;
             b.in = (pos & (p.c.page - 1)) >> 4;
             b.wanted = lane < kBlocks && pos < visible;
             if (b.wanted) b.id = __ldg(table + (pos >> p.c.page_shift));
-            x++, w.tile++;
+            b.some = true;
+            tile++;
             if (--left == 0) {
-                if (x < x1) next_segment(p, w);
-                open(x < x1);
+                next_segment(p, w);
+                open();
             }
             return b;
         };
@@ -808,11 +856,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const __grid_con
             }
             return b.id >= 0 ? __ldg(p.c.scale + (size_t)b.id * p.c.n_kv + b.head) : make_float2(0.f, 0.f);
         };
-        open(true);
+        open();
         Block b0 = ask_page(), b1 = ask_page();
         float2 sc = ask_scales(b0);
-        const unsigned count = (unsigned)(x1 - x0);
-        for (unsigned k = 0; k < count; k++) {
+        for (unsigned k = 0; b0.some; k++) {
             const Block b2 = ask_page();
             const float2 sc1 = ask_scales(b1);
             const bool there = b0.id >= 0, some = there && sc.y != 0.f;
@@ -843,8 +890,6 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const __grid_con
                 tqp::bulk_load(Cs + CODES + lane * TQ_KV_BLOCK * HDP, p.c.v + at, TQ_KV_BLOCK * HDP, &sh.code_full[1]);
             b0 = b1, b1 = b2, sc = sc1;
         }
-    } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(mma_regs(PIECES)));
     }
     __syncwarp();
     tqp::tc_fence_before();
@@ -861,13 +906,14 @@ template <int HDP, typename T>
 __global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const __grid_constant__ Params p, int grid) {
     __shared__ long long sums[kKvSums + 1];
     const long long total = list_sums<kJoinThreads>(p, sums);
-    const int G = (int)min((long long)grid, (total + kMinTiles - 1) / kMinTiles);
+    const int G = (int)min((long long)grid, (total + kMinUnits - 1) / kMinUnits);
     const int cta = blockIdx.x;
     if (cta + 1 >= G) return;
     const TqSplit split(total, G);
     const long long c0 = split.start(cta), c1 = split.start(cta + 1);
     const Where w = find(p, sums, c1 - 1);
-    if (w.from < c0 || w.from + w.tiles <= c1) return; // another CTA's, or whole
+    // its position tiles begin here and end elsewhere?
+    if (w.from < c0 || w.from >= c1 || w.from + w.tiles <= c1) return;
     const int k = split.owner(w.from + w.tiles - 1) - cta + 1;
     const float *part = reinterpret_cast<const float *>(static_cast<const char *>(p.a.workspace) + kKvHead);
     auto at = [&](int j) { return part + ((size_t)(cta + j) * 2 + (j == 0 ? 1 : 0)) * partial_floats(HDP); };
