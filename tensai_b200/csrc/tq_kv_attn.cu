@@ -39,6 +39,7 @@ using Params = TqKvParams;
 
 constexpr int kTile = 64;       // positions per step of a warp
 constexpr int kSlots = 3;       // ring slots per warp
+constexpr int kWide = 4;        // MMA accumulators worked on in turn
 constexpr int kMinTiles = 4;    // tiles per CTA below which fewer CTAs work
 constexpr int kPromptRows = 48; // rows of a sequence above which the prompt kernel takes it
 constexpr int kDirect = 1024;   // sequences whose lengths are kept in shared memory
@@ -326,17 +327,19 @@ __global__ void __launch_bounds__(32 * warps_of(HDP), ctas_of(HDP)) kv_attn_kern
                 for (int kk = 0; kk < KK; kk++) {
                     const int ch = HDP >= 128 ? (4 * kk + t) ^ ((g & 1) << 2) : 4 * kk + t;
 #pragma unroll
-                    for (int j = 0; j < 8; j++) {
-                        const uint4 w = *reinterpret_cast<const uint4 *>(ks + j * 2 * HDP + ch * 16);
-                        unsigned b0, b1;
-                        cvt4(w.x, b0, b1);
-                        mma16816(S[j], qf[kk][0], b0, b1);
-                        cvt4(w.y, b0, b1);
-                        mma16816(S[j], qf[kk][1], b0, b1);
-                        cvt4(w.z, b0, b1);
-                        mma16816(S[j], qf[kk][2], b0, b1);
-                        cvt4(w.w, b0, b1);
-                        mma16816(S[j], qf[kk][3], b0, b1);
+                    for (int j0 = 0; j0 < 8; j0 += kWide) { // kWide sums in turn: none waits for its last product
+                        uint4 w[kWide];
+#pragma unroll
+                        for (int j = 0; j < kWide; j++)
+                            w[j] = *reinterpret_cast<const uint4 *>(ks + (j0 + j) * 2 * HDP + ch * 16);
+#pragma unroll
+                        for (int u = 0; u < 4; u++)
+#pragma unroll
+                            for (int j = 0; j < kWide; j++) {
+                                unsigned b0, b1;
+                                cvt4((&w[j].x)[u], b0, b1);
+                                mma16816(S[j0 + j], qf[kk][u], b0, b1);
+                            }
                     }
                 }
             }
@@ -416,17 +419,18 @@ __global__ void __launch_bounds__(32 * warps_of(HDP), ctas_of(HDP)) kv_attn_kern
             {
                 const unsigned char *vs = ring + (used % kSlots) * slot_bytes(HDP) + t * value_pitch(HDP) + g * 16;
 #pragma unroll
-                for (int i = 0; i < NI; i++) {
-                    const uint4 w = *reinterpret_cast<const uint4 *>(vs + i * 128);
-                    unsigned b0, b1;
-                    cvt4(w.x, b0, b1);
-                    mma16816(O[i], pf[0], b0, b1);
-                    cvt4(w.y, b0, b1);
-                    mma16816(O[i], pf[1], b0, b1);
-                    cvt4(w.z, b0, b1);
-                    mma16816(O[i], pf[2], b0, b1);
-                    cvt4(w.w, b0, b1);
-                    mma16816(O[i], pf[3], b0, b1);
+                for (int i0 = 0; i0 < NI; i0 += kWide) {
+                    uint4 w[kWide];
+#pragma unroll
+                    for (int i = 0; i < kWide; i++) w[i] = *reinterpret_cast<const uint4 *>(vs + (i0 + i) * 128);
+#pragma unroll
+                    for (int u = 0; u < 4; u++)
+#pragma unroll
+                        for (int i = 0; i < kWide; i++) {
+                            unsigned b0, b1;
+                            cvt4((&w[i].x)[u], b0, b1);
+                            mma16816(O[i0 + i], pf[u], b0, b1);
+                        }
                 }
             }
             used++;
