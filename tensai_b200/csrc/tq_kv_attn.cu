@@ -23,9 +23,10 @@
 // fragments: sixteen dimensions of a key, or sixteen positions of a value
 // dimension, are one 16-byte read, and q and p are permuted to match. The scores
 // of the MMA's accumulator are the next product's operand in place.
-// All (sequence, KV head, row tile) segments laid end to end are cut evenly over
-// the CTAs, then over their warps, wherever the cuts fall (lengths are device
-// data; every CTA makes the same sums). A warp's unfinished segments meet in its
+// All (sequence, KV head, row tile) segments laid end to end, each as long as its
+// tiles and a unit before them for what it costs besides, are cut evenly over the
+// CTAs, then over their warps, wherever the cuts fall (lengths are device data;
+// every CTA makes the same sums). A warp's unfinished segments meet in its
 // CTA, the CTA's in the CTA that arrives last, in a fixed order: results do not
 // depend on timing.
 #include <climits>
@@ -40,7 +41,8 @@ using Params = TqKvParams;
 constexpr int kTile = 64;       // positions per step of a warp
 constexpr int kSlots = 3;       // ring slots per warp
 constexpr int kWide = 4;        // MMA accumulators worked on in turn
-constexpr int kMinTiles = 4;    // tiles per CTA below which fewer CTAs work
+constexpr int kSegCost = 1;     // what a segment costs besides its tiles, in tiles
+constexpr int kMinTiles = 8;    // units per CTA below which fewer CTAs work
 constexpr int kPromptRows = 48; // rows of a sequence above which the prompt kernel takes it
 constexpr int kDirect = 1024;   // sequences whose lengths are kept in shared memory
 constexpr int kSums = kKvSums;
@@ -48,20 +50,20 @@ constexpr float kPUnit = 16384.f; // p = 1 in float16: its low piece stays norma
 constexpr size_t kHead = kKvHead;
 constexpr int kMaxGrid = kHead / sizeof(unsigned);
 
-constexpr int warps_of(int hdp) { return hdp == 256 ? 4 : 8; }
-constexpr int ctas_of(int hdp) { return hdp == 64 ? 2 : 1; } // CTAs per SM
+constexpr int warps_of(int hdp) { return hdp == 256 ? 4 : hdp == 128 ? 8 : 12; } // one CTA per SM
 constexpr int slot_bytes(int hdp) { return kTile * hdp + 128; }
 constexpr int value_pitch(int hdp) { return TQ_KV_BLOCK * hdp + 32; } // four blocks in distinct banks
-constexpr int partial_floats(int hdp) { return 16 * (hdp + 2); }
-constexpr int partials_of(int hdp) { return 2 * warps_of(hdp) + 2; } // per CTA
+constexpr int partial_pitch(int hdp) { return hdp + 8; } // floats of a row: two wavefronts a store
+constexpr int partial_floats(int hdp) { return 16 * partial_pitch(hdp) + 32; } // sums, then m, then l
+constexpr int partials_of(int hdp) { return warps_of(hdp) + 2; } // per CTA: two that others read, one for each warp
 constexpr size_t smem_bytes(int hdp) {
     return (size_t)warps_of(hdp) * kSlots * slot_bytes(hdp) + sizeof(long long) * (kSums + 1) +
            sizeof(int) * (2 * kDirect + 2);
 }
 
 template <int HDP, int PIECES, typename T>
-__global__ void __launch_bounds__(32 * warps_of(HDP), ctas_of(HDP)) kv_attn_kernel(const __grid_constant__ Params p) {
-    constexpr int NW = warps_of(HDP), NT = 32 * NW, R = 16 / PIECES, KK = HDP / 64, NI = HDP / 8;
+__global__ void __launch_bounds__(32 * warps_of(HDP), 1) kv_attn_kernel(const __grid_constant__ Params p) {
+    constexpr int NW = warps_of(HDP), NT = 32 * NW, R = 16 / PIECES, KK = HDP / 64, NI = HDP / 8, PP = partial_pitch(HDP);
     extern __shared__ __align__(128) unsigned char sm[];
     long long *sums = reinterpret_cast<long long *>(sm + (size_t)NW * kSlots * slot_bytes(HDP));
     int *s_starts = reinterpret_cast<int *>(sums + kSums + 1), *s_lens = s_starts + kDirect + 1;
@@ -69,22 +71,29 @@ __global__ void __launch_bounds__(32 * warps_of(HDP), ctas_of(HDP)) kv_attn_kern
     __shared__ long long s_scan[NW + 1];
     __shared__ long long e_seg[2 * NW], e_end[2 * NW]; // unfinished segments of the warps: first and last tile + 1
     __shared__ int e_row[2 * NW][3];                   // their sequence, KV head, row tile
-    __shared__ volatile int s_late;
-    __shared__ int s_last;
+    __shared__ const float *e_at[2 * NW];              // and where their sums are
+    __shared__ int s_list[2 * NW], s_count;
+    __shared__ volatile int s_late[NW];
+    __shared__ int s_shared[2][3], s_last[2]; // segments that other CTAs share: their place here, first and last CTA
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const int n = p.a.n, n_kv = p.c.n_kv, group = p.group;
 
     // ---- lengths, checked; sums of the sequences' tiles --------------------------------
-    const bool direct = n <= kDirect;
+    // Up to 32 sequences: every warp makes the sums for itself, a sequence a lane.
+    // Else the block makes them, the lengths and sums in shared memory.
+    const bool alone = n <= 32, direct = !alone && n <= kDirect;
     if (direct) {
         for (int i = tid; i <= n; i += NT) s_starts[i] = p.a.starts[i];
         for (int i = tid; i < n; i += NT) s_lens[i] = p.a.lens[i];
     }
     if (lane < kSlots) tqp::mbar_init(&bars[warp][lane], 1);
-    if (tid == 0) s_late = 0;
-    if (tid < 2 * NW) e_seg[tid] = -1;
+    if (lane == 0) s_late[warp] = 0;
+    if (lane < 2) e_seg[2 * warp + lane] = -1;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    __syncthreads();
+    if (alone)
+        __syncwarp();
+    else
+        __syncthreads();
     const int *starts = direct ? s_starts : p.a.starts, *lens = direct ? s_lens : p.a.lens;
     auto seq_of = [&](int i) {
         Seq s = seq_at(p, starts, lens, i);
@@ -93,10 +102,25 @@ __global__ void __launch_bounds__(32 * warps_of(HDP), ctas_of(HDP)) kv_attn_kern
     };
     auto tiles_per = [](const Seq &s) { return s.len > kTile ? (s.len + kTile - 1) / kTile : 1; };
     auto row_tiles = [&](const Seq &s) { return (s.nq * group + R - 1) / R; };
+    auto units_of = [&](int nrt, int tps) { return (long long)nrt * n_kv * (tps + kSegCost); };
     const int span = 1 << p.shift_sums, entries = (n + span - 1) >> p.shift_sums;
-    long long total;
-    { // kSums entries over NT threads
-        constexpr int PER = kSums / NT;
+    long long total, lane_sum = 0; // lane_sum: units before sequence `lane`
+    if (alone) {
+        long long own = 0;
+        if (lane < n) {
+            const Seq s = seq_of(lane);
+            own = units_of(row_tiles(s), tiles_per(s));
+        }
+        long long inc = own;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long v = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += v;
+        }
+        lane_sum = inc - own;
+        total = __shfl_sync(0xffffffffu, inc, 31);
+    } else { // kSums entries over NT threads
+        constexpr int PER = (kSums + NT - 1) / NT;
         long long own[PER], sum = 0;
 #pragma unroll
         for (int u = 0; u < PER; u++) {
@@ -104,7 +128,7 @@ __global__ void __launch_bounds__(32 * warps_of(HDP), ctas_of(HDP)) kv_attn_kern
             own[u] = 0;
             for (int i = e << p.shift_sums; e < entries && i < min(n, (e + 1) << p.shift_sums); i++) {
                 const Seq s = seq_of(i);
-                own[u] += (long long)row_tiles(s) * n_kv * tiles_per(s);
+                own[u] += units_of(row_tiles(s), tiles_per(s));
             }
             sum += own[u];
         }
@@ -140,39 +164,54 @@ __global__ void __launch_bounds__(32 * warps_of(HDP), ctas_of(HDP)) kv_attn_kern
     const long long c0 = split.start(blockIdx.x), c1 = split.start(blockIdx.x + 1);
     const long long x0 = c0 + (c1 - c0) * warp / NW, x1 = c0 + (c1 - c0) * (warp + 1) / NW;
     float *part = reinterpret_cast<float *>(static_cast<char *>(p.a.workspace) + kHead);
-    auto partial_at = [&](int cta, int k) { return part + ((size_t)cta * partials_of(HDP) + k) * partial_floats(HDP); };
+    // what other CTAs read lies together: few memory pages to look up
+    auto partial_at = [&](int cta, int k) { return part + (size_t)(2 * cta + k) * partial_floats(HDP); };
+    auto warp_partial = [&]() {
+        return part + ((size_t)2 * gridDim.x + (size_t)NW * blockIdx.x + warp) * partial_floats(HDP);
+    };
 
-    struct Cursor {
-        int i, seg, tile, tps, nrt, nseg;
+    struct Cursor { // a segment (sequence, KV head, row tile) and a tile of it
+        int i, head, rt, nrt, tile, tps;
+        int seen;      // positions that some row of it sees
+        long long pos; // the tile's unit
         Seq s;
     };
     auto enter = [&](Cursor &c) { // a sequence's figures
         c.s = seq_of(c.i);
         c.tps = tiles_per(c.s);
         c.nrt = row_tiles(c.s);
-        c.nseg = c.nrt * n_kv;
     };
-    auto advance = [&](Cursor &c) {
+    auto begin = [&](Cursor &c) { // a segment's
+        const int last = min((c.rt + 1) * R, c.s.nq * group) - 1;
+        c.seen = min(c.s.len, max(0, c.s.len - c.s.nq + last / group + 1));
+    };
+    auto advance = [&](Cursor &c) { // to the next tile; its pos is at or past the list's end when there is none
+        c.pos++;
         if (++c.tile < c.tps) return;
         c.tile = 0;
-        if (++c.seg < c.nseg) return;
-        c.seg = 0;
-        do {
-            c.i++;
-            if (c.i >= n) return;
-            enter(c);
-        } while (c.nseg == 0);
-    };
-    // positions that some row of the cursor's segment sees
-    auto seen_by = [&](const Cursor &c) {
-        const int rt = c.seg % c.nrt, last = min((rt + 1) * R, c.s.nq * group) - 1;
-        return min(c.s.len, max(0, c.s.len - c.s.nq + last / group + 1));
+        c.pos += kSegCost;
+        if (++c.rt == c.nrt) {
+            c.rt = 0;
+            if (++c.head == n_kv) {
+                c.head = 0;
+                do {
+                    c.i++;
+                    if (c.i >= n) return;
+                    enter(c);
+                } while (c.nrt == 0);
+            }
+        }
+        begin(c);
     };
 
     unsigned char *ring = sm + (size_t)warp * kSlots * slot_bytes(HDP);
-    if (x0 < x1) {
-        Cursor cur;
-        {
+    Cursor cur;
+    if (x0 < x1) { // the first tile at or behind unit x0
+        long long rest;
+        if (alone) { // the last sequence that begins at or before it: the one that holds it, empty ones apart
+            cur.i = 31 - __clz(__ballot_sync(0xffffffffu, lane < n && lane_sum <= x0));
+            rest = x0 - __shfl_sync(0xffffffffu, lane_sum, cur.i);
+        } else {
             int lo = 0, hi = entries;
             while (hi - lo > 1) {
                 const int mid = (lo + hi) >> 1;
@@ -181,34 +220,42 @@ __global__ void __launch_bounds__(32 * warps_of(HDP), ctas_of(HDP)) kv_attn_kern
                 else
                     hi = mid;
             }
-            long long rest = x0 - sums[lo];
+            rest = x0 - sums[lo];
             cur.i = lo << p.shift_sums;
-            enter(cur);
-            while (rest >= (long long)cur.nseg * cur.tps) {
-                rest -= (long long)cur.nseg * cur.tps;
-                cur.i++;
-                enter(cur);
-            }
-            cur.seg = (int)(rest / cur.tps);
-            cur.tile = (int)(rest - (long long)cur.seg * cur.tps);
         }
+        enter(cur);
+        while (rest >= units_of(cur.nrt, cur.tps)) {
+            rest -= units_of(cur.nrt, cur.tps);
+            cur.i++;
+            enter(cur);
+        }
+        const int per = cur.tps + kSegCost, seg = (int)(rest / per), in = (int)(rest - (long long)seg * per);
+        cur.head = seg / cur.nrt;
+        cur.rt = seg - cur.head * cur.nrt;
+        cur.tile = max(0, in - kSegCost);
+        cur.pos = x0 + max(0, kSegCost - in);
+        begin(cur);
+    }
+    if (x0 < x1 && cur.pos < x1) {
         // ---- the loader: one tile's keys, then its values; item = 2 * tile number + (0 | 1) --
         Cursor ld = cur;
-        long long left = x1 - x0; // tiles still to be loaded
-        int nid = -1, vid = -1, n_head = 0, v_head = 0;
         unsigned item = 0;
-        auto fetch_id = [&]() { // the page of this lane's block (t) of the loader's tile
-            nid = -1;
-            if (left <= 0) return;
+        struct Next { // this lane's block (t) of a tile: its page (< 0: not there), KV head, place in the page
+            int id, head, in;
+            bool some; // whether there is such a tile
+        };
+        auto ask = [&]() { // the next tile's; its page is on its way
+            Next b{-1, 0, 0, ld.pos < x1};
+            if (!b.some) return b;
             const int pos = ld.tile * kTile + t * TQ_KV_BLOCK;
-            n_head = ld.seg / ld.nrt;
-            if (pos < seen_by(ld)) {
-                nid = p.a.table[(size_t)ld.i * p.a.table_stride + (pos >> p.c.page_shift)];
-                if (nid < 0 || nid >= p.c.n_pages) {
-                    nid = -1;
-                    atomicOr(p.c.status, TQ_KV_STATUS_PAGE);
-                }
+            b.head = ld.head;
+            b.in = (pos & (p.c.page - 1)) >> 4;
+            if (pos < ld.seen) {
+                b.id = p.a.table[(size_t)ld.i * p.a.table_stride + (pos >> p.c.page_shift)];
+                if ((unsigned)b.id >= (unsigned)p.c.n_pages) b.id = -2;
             }
+            advance(ld);
+            return b;
         };
         auto copy = [&](const int8_t *from, int id, int head, int in_page, int pitch) {
             const unsigned slot = item % kSlots;
@@ -221,105 +268,110 @@ __global__ void __launch_bounds__(32 * warps_of(HDP), ctas_of(HDP)) kv_attn_kern
                                &bars[warp][slot]);
             item++;
         };
-        int n_block = 0, v_block = 0;
+        Next n0 = ask(), n1 = ask(), nv = n0; // the next tiles for keys, the next for values
         auto load_keys = [&](float2 &sc) { // and this lane's block's scales; x < 0: a block that is not there
             sc = make_float2(-1.f, 0.f);
-            if (left <= 0) return;
-            n_block = ((ld.tile * kTile + t * TQ_KV_BLOCK) & (p.c.page - 1)) >> 4;
-            copy(p.c.k, nid, n_head, n_block, TQ_KV_BLOCK * HDP);
-            if (nid >= 0) sc = __ldg(p.c.scale + (size_t)nid * n_kv + n_head);
-            vid = nid, v_head = n_head, v_block = n_block;
-            left--;
-            if (left > 0) advance(ld);
-            fetch_id();
+            if (!n0.some) return;
+            if (n0.id == -2) atomicOr(p.c.status, TQ_KV_STATUS_PAGE);
+            copy(p.c.k, n0.id, n0.head, n0.in, TQ_KV_BLOCK * HDP);
+            if (n0.id >= 0) sc = __ldg(p.c.scale + (size_t)n0.id * n_kv + n0.head);
+            nv = n0, n0 = n1, n1 = ask();
         };
-        auto load_values = [&]() { copy(p.c.v, vid, v_head, v_block, value_pitch(HDP)); };
+        auto load_values = [&]() { copy(p.c.v, nv.id, nv.head, nv.in, value_pitch(HDP)); };
 
         float2 sc, sc_next;
-        fetch_id();
-        load_keys(sc);
-        load_values();
-        load_keys(sc_next);
         unsigned used = 0; // items used
 
         unsigned qf[KK][4][4];
         float O[NI][4];
         float m[2], l[2], C = 0.f, row_unit[2];
         int lim[2], least = 0;
-        bool fresh = true;
         long long seg_from = 0;
-        const long long ntile = x1 - x0;
-        for (long long x = 0; x < ntile; x++) {
-            const int head = cur.seg / cur.nrt, rt = cur.seg - head * cur.nrt;
-            if (fresh) {
-                fresh = false;
-                seg_from = x0 + x - cur.tile;
-                const int rows = cur.s.nq * group;
-                least = cur.s.len;
+        auto start = [&](const Cursor &now) { // a segment: its queries, and nothing seen yet
+            seg_from = now.pos - now.tile;
+            least = min(now.s.len, max(0, now.s.len - now.s.nq + now.rt * R / group + 1));
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    m[h] = -INFINITY;
-                    l[h] = 0.f;
-                    row_unit[h] = 1.f;
-                    lim[h] = cur.s.len;
-                }
-                C = 0.f;
+            for (int h = 0; h < 2; h++) {
+                m[h] = -INFINITY;
+                l[h] = 0.f;
+                row_unit[h] = 1.f;
+                lim[h] = now.s.len;
+            }
+            C = 0.f;
 #pragma unroll
-                for (int i = 0; i < NI; i++) O[i][0] = O[i][1] = O[i][2] = O[i][3] = 0.f;
-                least = min(cur.s.len, max(0, cur.s.len - cur.s.nq + rt * R / group + 1));
+            for (int i = 0; i < NI; i++) O[i][0] = O[i][1] = O[i][2] = O[i][3] = 0.f;
 #pragma unroll
-                for (int h = 0; h < 3 - PIECES; h++) { // MMA rows g and, with one piece, g + 8
-                    const int row = rt * R + g + 8 * h;
-                    const int tok = row / group, hq = head * group + row - tok * group;
-                    const bool live = row < rows;
-                    float x[KK][16];
-                    float big = 0.f;
-                    const T *q = static_cast<const T *>(p.a.q) + (size_t)(cur.s.start + tok) * p.a.q_stride +
-                                 (size_t)hq * p.c.hd;
+            for (int h = 0; h < 3 - PIECES; h++) { // MMA rows g and, with one piece, g + 8
+                const int row = now.rt * R + g + 8 * h;
+                const int tok = row / group, hq = now.head * group + row - tok * group;
+                const bool live = row < now.s.nq * group;
+                const T *q = static_cast<const T *>(p.a.q) + (size_t)(now.s.start + tok) * p.a.q_stride +
+                             (size_t)hq * p.c.hd + 16 * t;
+                constexpr int E = 16 / sizeof(T), W = 16 / E; // words of the lane's sixteen dimensions
+                uint4 x[KK][W];
+                if (p.vec) {
 #pragma unroll
                     for (int kk = 0; kk < KK; kk++)
 #pragma unroll
-                        for (int j = 0; j < 2; j++) {
-                            const int d = 64 * kk + 16 * t + 8 * j;
-                            float y[8];
-                            if (live && d < p.c.hd)
-                                load8(q + d, p.vec, y);
-                            else
+                        for (int j = 0; j < W; j++)
+                            x[kk][j] = live && 64 * kk + 16 * t + E * j < p.c.hd
+                                           ? __ldg(reinterpret_cast<const uint4 *>(q + 64 * kk + E * j))
+                                           : make_uint4(0, 0, 0, 0);
+                } else {
 #pragma unroll
-                                for (int u = 0; u < 8; u++) y[u] = 0.f;
+                    for (int kk = 0; kk < KK; kk++)
 #pragma unroll
-                            for (int u = 0; u < 8; u++) {
-                                x[kk][8 * j + u] = y[u];
-                                big = fmaxf(big, fabsf(y[u]));
+                        for (int j = 0; j < W; j++)
+#pragma unroll
+                            for (int u = 0; u < E; u++)
+                                reinterpret_cast<T *>(&x[kk][j])[u] =
+                                    live && 64 * kk + 16 * t + E * j < p.c.hd ? q[64 * kk + E * j + u] : T(0.f);
+                }
+                float big = 0.f;
+#pragma unroll
+                for (int kk = 0; kk < KK; kk++)
+#pragma unroll
+                    for (int u = 0; u < 16; u++)
+                        big = fmaxf(big, fabsf(Elem<T>::get(reinterpret_cast<const T *>(&x[kk][0]) + u)));
+                big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+                big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+                const float unit = row_scale(big, &row_unit[h]);
+                if (live) lim[h] = min(now.s.len, max(0, now.s.len - now.s.nq + tok + 1));
+#pragma unroll
+                for (int kk = 0; kk < KK; kk++)
+#pragma unroll
+                    for (int u = 0; u < 4; u++)
+#pragma unroll
+                        for (int e = 0; e < 2; e++) { // dimensions 4u + 2e, + 1 of the lane's sixteen
+                            const T *y = reinterpret_cast<const T *>(&x[kk][0]) + 4 * u + 2 * e;
+                            const float y0 = Elem<T>::get(y) * unit, y1 = Elem<T>::get(y + 1) * unit;
+                            const unsigned hi = pack2(y0, y1);
+                            qf[kk][u][2 * e + h] = hi;
+                            if (PIECES == 2) {
+                                const float2 b = unpack2(hi);
+                                qf[kk][u][2 * e + 1] = pack2(y0 - b.x, y1 - b.y);
                             }
                         }
-                    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
-                    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
-                    const float unit = row_scale(big, &row_unit[h]);
-                    if (live) lim[h] = min(cur.s.len, max(0, cur.s.len - cur.s.nq + tok + 1));
-#pragma unroll
-                    for (int kk = 0; kk < KK; kk++)
-#pragma unroll
-                        for (int u = 0; u < 4; u++)
-#pragma unroll
-                            for (int e = 0; e < 2; e++) { // dimensions 4u + 2e, + 1 of the lane's sixteen
-                                const float y0 = x[kk][4 * u + 2 * e] * unit, y1 = x[kk][4 * u + 2 * e + 1] * unit;
-                                const unsigned hi = pack2(y0, y1);
-                                qf[kk][u][2 * e + h] = hi;
-                                if (PIECES == 2) {
-                                    const float2 b = unpack2(hi);
-                                    qf[kk][u][2 * e + 1] = pack2(y0 - b.x, y1 - b.y);
-                                }
-                            }
-                }
-                if (PIECES == 2) lim[1] = lim[0];
             }
+            if (PIECES == 2) lim[1] = lim[0];
+        };
+        start(cur);
+        load_keys(sc);
+        load_values();
+        load_keys(sc_next);
+        for (bool more = true, fresh = false; more;) {
+            const int head = cur.head, rt = cur.rt;
+            const Cursor now = cur;
+            advance(cur);
+            more = cur.pos < x1;
+            if (fresh) start(now);
+            fresh = false;
             // ---- s = q . k for 64 positions ----
-            const int pos0 = cur.tile * kTile;
+            const int pos0 = now.tile * kTile;
             float S[8][4];
 #pragma unroll
             for (int j = 0; j < 8; j++) S[j][0] = S[j][1] = S[j][2] = S[j][3] = 0.f;
-            wait_slot(&bars[warp][used % kSlots], (used / kSlots) & 1, &s_late, p.c.status);
+            wait_slot(&bars[warp][used % kSlots], (used / kSlots) & 1, &s_late[warp], p.c.status);
             {
                 const unsigned char *ks = ring + (used % kSlots) * slot_bytes(HDP) + (g >> 1) * TQ_KV_BLOCK * HDP +
                                           (g & 1) * HDP;
@@ -345,7 +397,7 @@ __global__ void __launch_bounds__(32 * warps_of(HDP), ctas_of(HDP)) kv_attn_kern
             }
             used++;
             __syncwarp(); // the slot is read
-            if (x + 1 < ntile) load_values();
+            if (more) load_values();
             // ---- softmax of the lane's 16 positions (its block), per row ----
             const bool there = sc.x >= 0.f || sc.x != sc.x;
             const bool whole = pos0 + kTile <= least && __all_sync(0xffffffffu, there);
@@ -415,7 +467,7 @@ __global__ void __launch_bounds__(32 * warps_of(HDP), ctas_of(HDP)) kv_attn_kern
                 }
             }
             // ---- O += p v ----
-            wait_slot(&bars[warp][used % kSlots], (used / kSlots) & 1, &s_late, p.c.status);
+            wait_slot(&bars[warp][used % kSlots], (used / kSlots) & 1, &s_late[warp], p.c.status);
             {
                 const unsigned char *vs = ring + (used % kSlots) * slot_bytes(HDP) + t * value_pitch(HDP) + g * 16;
 #pragma unroll
@@ -438,8 +490,8 @@ __global__ void __launch_bounds__(32 * warps_of(HDP), ctas_of(HDP)) kv_attn_kern
             sc = sc_next;
             load_keys(sc_next);
             // ---- the segment's end, or the warp's ----
-            const bool ends = cur.tile + 1 == cur.tps;
-            if (ends || x + 1 == ntile) {
+            const bool ends = now.tile + 1 == now.tps;
+            if (ends || !more) {
                 const float unit = C / kPUnit;
 #pragma unroll
                 for (int h = 0; h < H; h++) {
@@ -447,14 +499,14 @@ __global__ void __launch_bounds__(32 * warps_of(HDP), ctas_of(HDP)) kv_attn_kern
                     l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
                 }
                 const bool began = seg_from >= x0;
-                const int rows = cur.s.nq * group;
+                const int rows = now.s.nq * group;
                 if (ends && began) {
 #pragma unroll
                     for (int h = 0; h < H; h++) {
                         const int row = rt * R + g + 8 * h;
                         if (row >= rows) continue;
                         const int tok = row / group, hq = head * group + row - tok * group;
-                        T *o = static_cast<T *>(p.a.out) + (size_t)(cur.s.start + tok) * p.a.out_stride +
+                        T *o = static_cast<T *>(p.a.out) + (size_t)(now.s.start + tok) * p.a.out_stride +
                                (size_t)hq * p.c.hd;
                         const float inv = l[h] == 0.f ? 0.f : unit / l[h];
 #pragma unroll
@@ -466,62 +518,145 @@ __global__ void __launch_bounds__(32 * warps_of(HDP), ctas_of(HDP)) kv_attn_kern
                         }
                     }
                 } else { // to be joined: sums in plain units, m and l
-                    const int k = began ? 1 : 0, e = 2 * warp + k;
-                    float *to = partial_at(blockIdx.x, e);
+                    // the warp's last: over its ring, which is through; else the workspace
+                    const int e = 2 * warp + (began ? 1 : 0);
+                    float *to = !more ? reinterpret_cast<float *>(ring) : warp_partial();
 #pragma unroll
                     for (int h = 0; h < H; h++) {
 #pragma unroll
                         for (int i = 0; i < NI; i++) {
                             const float y0 = PIECES == 2 ? O[i][0] + O[i][2] : O[i][2 * h];
                             const float y1 = PIECES == 2 ? O[i][1] + O[i][3] : O[i][2 * h + 1];
-                            *reinterpret_cast<float2 *>(to + (g + 8 * h) * HDP + 8 * i + 2 * t) =
+                            *reinterpret_cast<float2 *>(to + (g + 8 * h) * PP + 8 * i + 2 * t) =
                                 make_float2(y0 * unit, y1 * unit);
                         }
                         if (t == 0) {
-                            to[16 * HDP + g + 8 * h] = m[h];
-                            to[16 * HDP + 16 + g + 8 * h] = l[h];
+                            to[16 * PP + g + 8 * h] = m[h];
+                            to[16 * PP + 16 + g + 8 * h] = l[h];
                         }
                     }
                     if (lane == 0) {
                         e_seg[e] = seg_from;
-                        e_end[e] = seg_from + cur.tps;
-                        e_row[e][0] = cur.i;
+                        e_end[e] = seg_from + now.tps;
+                        e_row[e][0] = now.i;
                         e_row[e][1] = head;
                         e_row[e][2] = rt;
+                        e_at[e] = to;
                     }
                 }
                 fresh = true;
             }
-            if (x + 1 < ntile) advance(cur);
         }
     }
     __syncthreads();
 
     // ---- join the warps' unfinished segments, then the CTAs' ------------------------------
-    // Sum of the partials `at(0..k)`; thread: 4 dimensions of a row at a time.
-    auto join = [&](auto at, int k, int i, int head, int rt, float *to) {
+    // the places in use, in order: a segment's are neighbours
+    if (warp == 0) {
+        const bool used = lane < 2 * NW && e_seg[lane] >= 0;
+        const unsigned all = __ballot_sync(0xffffffffu, used);
+        if (used) s_list[__popc(all & ((1u << lane) - 1))] = lane;
+        if (lane == 0) s_count = __popc(all);
+    }
+    __syncthreads();
+    // Job after job, one piece of code: the segments of this CTA; then, once it has
+    // arrived for those that others share (two at most, the first and the last),
+    // those that it was the last to arrive for.
+    const float **ptr = reinterpret_cast<const float **>(sm + sizeof(float) * partial_floats(HDP)); // over warp 0's ring
+    unsigned *counters = static_cast<unsigned *>(p.a.workspace);
+    int a = 0, shared = 0, done = -1;
+    for (;;) {
+        int k, i, head, rt;
+        float *to = nullptr; // where the sum goes: a partial, or the output
+        if (a < s_count) {
+            const int e = s_list[a];
+            const long long seg = e_seg[e], end = e_end[e];
+            for (k = 1; a + k < s_count && e_seg[s_list[a + k]] == seg; k++) {
+            }
+            i = e_row[e][0], head = e_row[e][1], rt = e_row[e][2];
+            if (tid < k) ptr[tid] = e_at[s_list[a + tid]];
+            if (seg < c0 || end > c1) {
+                const int first = split.owner(seg);
+                to = partial_at(blockIdx.x, (int)blockIdx.x == first ? 1 : 0);
+                if (tid == 0) s_shared[shared][0] = e, s_shared[shared][1] = first, s_shared[shared][2] = split.owner(end - 1);
+                shared++;
+            }
+            a += k;
+        } else {
+            if (shared == 0) break;
+            if (done < 0) {
+                __syncthreads(); // the partials are written
+                if (tid < shared)
+                    s_last[tid] = tq_arrive_last(counters + s_shared[tid][1], s_shared[tid][2] - s_shared[tid][1] + 1);
+                __syncthreads();
+                done = 0;
+            }
+            while (done < shared && !s_last[done]) done++;
+            if (done == shared) break;
+            const int e = s_shared[done][0], first = s_shared[done][1];
+            k = s_shared[done][2] - first + 1;
+            i = e_row[e][0], head = e_row[e][1], rt = e_row[e][2];
+            done++;
+        }
+        __syncthreads();
+        // the sum of the k partials; a thread: 4 dimensions of a row at a time, kAhead partials on their way
+        constexpr int kAhead = 8;
         const Seq s = seq_of(i);
         const int rows = min(R, s.nq * group - rt * R);
         for (int e = tid; e < rows * (HDP / 4); e += NT) {
             const int r = e / (HDP / 4), d = (e - r * (HDP / 4)) * 4;
-            float M = -INFINITY;
-            for (int j = 0; j < k; j++) M = fmaxf(M, __ldcg(at(j) + 16 * HDP + r));
-            const float base = M == -INFINITY ? 0.f : M;
-            float L = 0.f;
+            float M = -INFINITY, L = 0.f;
             float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (int j = 0; j < k; j++) {
-                const float *f = at(j);
-                const float w = exp2f(__ldcg(f + 16 * HDP + r) - base);
-                const float4 y = __ldcg(reinterpret_cast<const float4 *>(f + r * HDP + d));
-                L += w * __ldcg(f + 16 * HDP + 16 + r);
-                A.x += w * y.x;
-                A.y += w * y.y;
-                A.z += w * y.z;
-                A.w += w * y.w;
+            auto add = [&](const float (&m)[kAhead], const float (&l)[kAhead], const float4 (&y)[kAhead]) {
+                float top = M;
+#pragma unroll
+                for (int u = 0; u < kAhead; u++) top = fmaxf(top, m[u]);
+                const float base = top == -INFINITY ? 0.f : top, old = exp2f(M - base);
+                M = top;
+                L *= old, A.x *= old, A.y *= old, A.z *= old, A.w *= old;
+#pragma unroll
+                for (int u = 0; u < kAhead; u++) {
+                    const float w = exp2f(m[u] - base);
+                    L += w * l[u];
+                    A.x += w * y[u].x;
+                    A.y += w * y[u].y;
+                    A.z += w * y[u].z;
+                    A.w += w * y[u].w;
+                }
+            };
+            float m[kAhead], l[kAhead];
+            float4 y[kAhead];
+            if (done < 0) { // this CTA's: in shared memory, but for some in the workspace
+#pragma unroll 1
+                for (int j0 = 0; j0 < k; j0 += kAhead) {
+#pragma unroll
+                    for (int u = 0; u < kAhead; u++) { // the last again, at no weight, beyond the end
+                        const float *f = ptr[min(j0 + u, k - 1)];
+                        m[u] = f[16 * PP + r];
+                        l[u] = f[16 * PP + 16 + r];
+                        y[u] = *reinterpret_cast<const float4 *>(f + r * PP + d);
+                        if (j0 + u >= k) m[u] = -INFINITY;
+                    }
+                    add(m, l, y);
+                }
+            } else {
+#pragma unroll 1
+                for (int j0 = 0; j0 < k; j0 += kAhead) {
+#pragma unroll
+                    for (int u = 0; u < kAhead; u++) {
+                        const int j = min(j0 + u, k - 1);
+                        const float *f = partial_at(s_shared[done - 1][1] + j, j == 0 ? 1 : 0);
+                        m[u] = __ldcg(f + 16 * PP + r);
+                        l[u] = __ldcg(f + 16 * PP + 16 + r);
+                        y[u] = __ldcg(reinterpret_cast<const float4 *>(f + r * PP + d));
+                        if (j0 + u >= k) m[u] = -INFINITY;
+                    }
+                    add(m, l, y);
+                }
             }
             if (to) {
-                *reinterpret_cast<float4 *>(to + r * HDP + d) = A;
-                if (d == 0) to[16 * HDP + r] = M, to[16 * HDP + 16 + r] = L;
+                *reinterpret_cast<float4 *>(to + r * PP + d) = A;
+                if (d == 0) to[16 * PP + r] = M, to[16 * PP + 16 + r] = L;
             } else if (d < p.c.hd) {
                 const int row = rt * R + r, tok = row / group, hq = head * group + row - tok * group;
                 T *o = static_cast<T *>(p.a.out) + (size_t)(s.start + tok) * p.a.out_stride + (size_t)hq * p.c.hd + d;
@@ -530,37 +665,7 @@ __global__ void __launch_bounds__(32 * warps_of(HDP), ctas_of(HDP)) kv_attn_kern
                 Elem<T>::put2(o + 2, A.z * inv, A.w * inv, p.vec, true);
             }
         }
-    };
-    unsigned *counters = static_cast<unsigned *>(p.a.workspace);
-    for (int e = 0; e < 2 * NW;) {
-        const long long seg = e_seg[e];
-        if (seg < 0) {
-            e++;
-            continue;
-        }
-        // the run of partials of this segment (empty places between them are skipped)
-        int list[2 * NW], k = 0, f = e;
-        for (; f < 2 * NW; f++) {
-            if (e_seg[f] < 0) continue;
-            if (e_seg[f] != seg) break;
-            list[k++] = f;
-        }
-        const long long end = e_end[e];
-        const int i = e_row[e][0], head = e_row[e][1], rt = e_row[e][2];
-        auto mine = [&](int j) -> const float * { return partial_at(blockIdx.x, list[j]); };
-        if (seg >= c0 && end <= c1) {
-            join(mine, k, i, head, rt, nullptr);
-        } else {
-            const int first = split.owner(seg), last = split.owner(end - 1);
-            join(mine, k, i, head, rt, partial_at(blockIdx.x, 2 * NW + ((int)blockIdx.x == first ? 1 : 0)));
-            __syncthreads();
-            if (tid == 0) s_last = tq_arrive_last(counters + first, last - first + 1);
-            __syncthreads();
-            if (s_last)
-                join([&](int j) -> const float * { return partial_at(first + j, 2 * NW + (j == 0 ? 1 : 0)); },
-                     last - first + 1, i, head, rt, nullptr);
-        }
-        e = f;
+        __syncthreads(); // the pointers are read
     }
 }
 
@@ -575,7 +680,7 @@ cudaError_t launch(const Params &p, int sms, cudaStream_t st) {
                                         (int)smem_bytes(HDP));
         });
     if (e != cudaSuccess) return e;
-    const int grid = min(kMaxGrid, sms * ctas_of(HDP));
+    const int grid = min(kMaxGrid, sms);
     kv_attn_kernel<HDP, PIECES, T><<<grid, 32 * warps_of(HDP), smem_bytes(HDP), st>>>(p);
     return cudaGetLastError();
 }
@@ -592,7 +697,7 @@ template <int HDP> cudaError_t launch_hd(const Params &p, int sms, cudaStream_t 
 } // namespace
 
 static size_t small_workspace(int hdp, int sms) {
-    const size_t grid = (size_t)(sms * ctas_of(hdp) < kMaxGrid ? sms * ctas_of(hdp) : kMaxGrid);
+    const size_t grid = (size_t)(sms < kMaxGrid ? sms : kMaxGrid);
     return kHead + grid * partials_of(hdp) * partial_floats(hdp) * sizeof(float);
 }
 size_t tq_kv_attn_workspace(int hdp, int sms) {
