@@ -24,65 +24,121 @@
 
 namespace {
 
-constexpr int kStoreThreads = 128;
+constexpr int kStoreThreads = 256; // or 128 for little pages
+constexpr int kStoreWarps = kStoreThreads / 32;
 constexpr int kMaxPage = 128;
-static_assert(kStoreThreads >= kMaxPage, "one thread per token of a run");
+static_assert(kStoreThreads / 2 >= kMaxPage, "one thread per token of a run");
+constexpr float kRound = 12582912.f; // 1.5 * 2^23: x + kRound holds the integer nearest to x in its low bits
 
 __device__ __forceinline__ float to_f(float x) { return x; }
 __device__ __forceinline__ float to_f(__half x) { return __half2float(x); }
 __device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
 
 // The integer nearest to x / s (ties to even), |x| <= 127 s up to rounding.
-__device__ __forceinline__ int code_of(float x, float s, float inv) {
+__device__ __noinline__ unsigned code_exact(float x, float s, float inv) {
     if (!(s > 0.f)) return 0; // zero or NaN
     if (s < 0x1p-100f)        // the products below could underflow
-        return (int)fmin(fmax(rint(__ddiv_rn((double)x, (double)s)), -127.0), 127.0);
-    const float y = __fmul_rn(x, inv);
+        return (unsigned)(int)fmin(fmax(rint(__ddiv_rn((double)x, (double)s)), -127.0), 127.0);
+    const float y = __fmul_rn(x, inv), lo = floorf(y);
     float t = rintf(y);
-    if (fabsf(y - t) > 0.4999f) {
-        const float lo = floorf(y); // the half between lo and lo + 1 decides
+    if (fabsf(y - t) > 0.4999f) { // the half between lo and lo + 1 decides
         const float r = __fmaf_rn(-(lo + 0.5f), s, x);
         t = r > 0.f ? lo + 1.f : r < 0.f ? lo : 2.f * rintf(0.5f * (lo + 0.5f));
     }
-    return (int)fminf(fmaxf(t, -127.f), 127.f);
+    return (unsigned)(int)fminf(fmaxf(t, -127.f), 127.f);
+}
+
+// Four codes, a byte each. easy: the scale is neither zero, NaN nor tiny.
+__device__ __forceinline__ unsigned codes4(const float (&x)[4], float s, float inv, bool easy) {
+    float v[4], off = easy ? 0.f : 1.f;
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+        const float y = __fmul_rn(x[u], inv);
+        v[u] = __fadd_rn(y, kRound);
+        off = fmaxf(off, fabsf(__fadd_rn(y, -__fadd_rn(v[u], -kRound)))); // from the nearest integer
+    }
+    if (off > 0.4999f) // rare: next to a half
+        return (code_exact(x[0], s, inv) & 0xffu) | (code_exact(x[1], s, inv) & 0xffu) << 8 |
+               (code_exact(x[2], s, inv) & 0xffu) << 16 | code_exact(x[3], s, inv) << 24;
+    return __byte_perm(__byte_perm(__float_as_uint(v[0]), __float_as_uint(v[1]), 0x0040),
+                       __byte_perm(__float_as_uint(v[2]), __float_as_uint(v[3]), 0x0040), 0x5410);
 }
 
 // The integer nearest to c * was / now (ties to even).
-__device__ __forceinline__ int recode(int c, float was, float now, float ratio) {
-    const float y = __fmul_rn((float)c, ratio), t = rintf(y);
-    if (fabsf(y - t) > 0.4999f) return (int)rint(__ddiv_rn((double)c * (double)was, (double)now));
-    return (int)t;
+__device__ __forceinline__ unsigned recode(unsigned byte, float was, float now, float ratio) {
+    const float c = (float)(int8_t)byte, y = __fmul_rn(c, ratio), v = __fadd_rn(y, kRound);
+    if (fabsf(__fadd_rn(y, -__fadd_rn(v, -kRound))) > 0.4999f)
+        return (unsigned)(int)rint(__ddiv_rn((double)c * (double)was, (double)now)) & 0xffu;
+    return __float_as_uint(v) & 0xffu;
+}
+__device__ __noinline__ unsigned recode4(unsigned w, float was, float now, float ratio) {
+    return recode(w & 0xffu, was, now, ratio) | recode(w >> 8 & 0xffu, was, now, ratio) << 8 |
+           recode(w >> 16 & 0xffu, was, now, ratio) << 16 | recode(w >> 24, was, now, ratio) << 24;
+}
+
+// e / per and e % per for e = threadIdx.x, + blockDim.x, ..: one division, then steps.
+struct Places {
+    int q, r, dq, dr, per;
+    __device__ __forceinline__ explicit Places(int n) : per(n) {
+        q = threadIdx.x / per, r = threadIdx.x - q * per;
+        dq = blockDim.x / per, dr = blockDim.x - dq * per;
+    }
+    __device__ __forceinline__ void step() {
+        q += dq, r += dr;
+        if (r >= per) r -= per, q++;
+    }
+};
+
+// Two neighbouring elements, widened.
+__device__ __forceinline__ float2 pair_at(const float *p) { return *reinterpret_cast<const float2 *>(p); }
+__device__ __forceinline__ float2 pair_at(const __half *p) { return __half22float2(*reinterpret_cast<const __half2 *>(p)); }
+__device__ __forceinline__ float2 pair_at(const __nv_bfloat16 *p) {
+    return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(p));
+}
+// Eight, 16-byte aligned.
+template <typename T> __device__ __forceinline__ void eight_at(const T *p, float (&x)[8]) {
+    constexpr int E = 16 / sizeof(T);
+#pragma unroll
+    for (int j = 0; j < 8 / E; j++) {
+        const uint4 w = *reinterpret_cast<const uint4 *>(p + j * E);
+#pragma unroll
+        for (int u = 0; u < E; u++) x[j * E + u] = to_f(reinterpret_cast<const T *>(&w)[u]);
+    }
 }
 
 __device__ __forceinline__ unsigned byte_of(unsigned w, int i) { return (w >> (8 * i)) & 0xffu; }
 
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(kStoreThreads) kv_store_kernel(TqKvView c, const T *k, const T *v, long long k_stride,
+__global__ void __launch_bounds__(kStoreThreads, 4) kv_store_kernel(TqKvView c, const T *k, const T *v, long long k_stride,
                                                                  long long v_stride, const long long *slots, int n,
                                                                  int window) {
     extern __shared__ __align__(16) unsigned char store_sm[];
     T *xs = reinterpret_cast<T *>(store_sm); // [run][hd]
-    __shared__ unsigned s_max[kStoreThreads / 32];
-    __shared__ int s_run[kStoreThreads / 32];
+    __shared__ unsigned s_max[kStoreWarps];
+    __shared__ int s_run[kStoreWarps];
     const int head = blockIdx.y, side = blockIdx.z, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int P = c.page, hd = c.hd, hdp = c.hdp;
     const T *src = side ? v : k;
     const long long stride = side ? v_stride : k_stride, most = (long long)c.n_pages << c.page_shift;
     int8_t *codes = side ? c.v : c.k;
-    const int t1 = min(n, (int)(blockIdx.x + 1) * window);
-    for (int t = blockIdx.x * window; t < t1; t++) {
-        const long long slot = slots[t];
-        if (slot < 0) continue; // skipped by the caller, or by a plan that failed
-        if (slot >= most) {
-            if (tid == 0) atomicOr(c.status, TQ_KV_STATUS_PAGE);
-            continue;
-        }
-        const long long before = t ? slots[t - 1] : -1;
+    // the tokens of this window that begin a run: a lane each, in every warp
+    const int t0 = blockIdx.x * window, mine = t0 + lane;
+    unsigned firsts;
+    const long long lane_slot = lane < window && mine < n ? slots[mine] : -1;
+    {
+        const long long slot = lane_slot, before = lane < window && mine < n && mine ? slots[mine - 1] : -1;
+        const bool there = slot >= 0 && slot < most; // negative: skipped by the caller, or by a plan that failed
+        const bool goes_on = there && before >= 0 && (before >> c.page_shift) == (slot >> c.page_shift);
+        if (warp == 0 && slot >= most) atomicOr(c.status, TQ_KV_STATUS_PAGE);
+        if (warp == 0 && goes_on && before + 1 != slot) atomicOr(c.status, TQ_KV_STATUS_SLOTS);
+        firsts = __ballot_sync(0xffffffffu, there && !goes_on);
+    }
+    for (; firsts; firsts &= firsts - 1) {
+        const int t = t0 + __ffs(firsts) - 1;
+        const long long slot = __shfl_sync(0xffffffffu, lane_slot, t - t0);
         const int id = (int)(slot >> c.page_shift), off = (int)slot & (P - 1);
-        if (before >= 0 && (before >> c.page_shift) == id) { // not the first of its run
-            if (before + 1 != slot && tid == 0) atomicOr(c.status, TQ_KV_STATUS_SLOTS);
-            continue;
-        }
+        float *place = reinterpret_cast<float *>(c.scale + (size_t)id * c.n_kv + head) + side;
+        const float held = off ? *place : 0.f;
         // the run's length: tokens t, t + 1, .. in slots slot, slot + 1, .. of this page
         const bool in = tid < P - off && tid < n - t && slots[t + tid] == slot + tid;
         const unsigned miss = ~__ballot_sync(0xffffffffu, in);
@@ -90,26 +146,26 @@ __global__ void __launch_bounds__(kStoreThreads) kv_store_kernel(TqKvView c, con
         __syncthreads();
         int run = s_run[0];
 #pragma unroll
-        for (int w = 1; w < kStoreThreads / 32; w++)
+        for (int w = 1; w < kMaxPage / 32; w++)
             if (run == 32 * w) run += s_run[w];
         // the run into shared memory, and its largest magnitude
         unsigned mx = 0;
         const T *base = src + (size_t)t * stride + (size_t)head * hd;
         if (VEC) {
             constexpr int E = 16 / sizeof(T);
-            const int per = hd / E;
-            for (int e = tid; e < run * per; e += kStoreThreads) {
-                const int r = e / per, j = e - r * per;
-                uint4 w = *reinterpret_cast<const uint4 *>(base + (size_t)r * stride + j * E);
-                *reinterpret_cast<uint4 *>(xs + r * hd + j * E) = w;
+            Places at(hd / E);
+#pragma unroll 4
+            for (int e = tid; e < run * at.per; e += blockDim.x, at.step()) {
+                const uint4 w = *reinterpret_cast<const uint4 *>(base + (size_t)at.q * stride + at.r * E);
+                *reinterpret_cast<uint4 *>(xs + e * E) = w;
                 const T *x = reinterpret_cast<const T *>(&w);
 #pragma unroll
                 for (int u = 0; u < E; u++) mx = max(mx, __float_as_uint(to_f(x[u])) & 0x7fffffffu);
             }
         } else {
-            for (int e = tid; e < run * hd; e += kStoreThreads) {
-                const int r = e / hd, j = e - r * hd;
-                const T x = base[(size_t)r * stride + j];
+            Places at(hd);
+            for (int e = tid; e < run * hd; e += blockDim.x, at.step()) {
+                const T x = base[(size_t)at.q * stride + at.r];
                 xs[e] = x;
                 mx = max(mx, __float_as_uint(to_f(x)) & 0x7fffffffu);
             }
@@ -118,65 +174,81 @@ __global__ void __launch_bounds__(kStoreThreads) kv_store_kernel(TqKvView c, con
         if (lane == 0) s_max[warp] = mx;
         __syncthreads();
 #pragma unroll
-        for (int w = 0; w < kStoreThreads / 32; w++) mx = max(mx, s_max[w]);
-        float *place = reinterpret_cast<float *>(c.scale + (size_t)id * c.n_kv + head) + side;
+        for (int w = 0; w < kStoreWarps; w++)
+            if (w < (int)blockDim.x >> 5) mx = max(mx, s_max[w]);
         float now = mx < 0x7f800000u ? __fdiv_rn(__uint_as_float(mx), 127.f) : __uint_as_float(0x7fc00000u);
-        const float was = off ? *place : 0.f;
+        const float was = held;
         if (off && !(now >= was)) now = now != now ? now : was; // the larger; a NaN stays
-        const bool grew = off && now != was && now == now;
+        const bool grew = off && now != was && now == now, easy = now >= 0x1p-100f;
         const float inv = __fdiv_rn(1.f, now), ratio = __fdiv_rn(was, now);
         int8_t *page = codes + kv_block_offset(c, id, head, 0);
         const int end = off + run;
         if (side == 0) {
-            const int chunks = hdp / 16;
-            for (int e = tid + (grew ? 0 : off * chunks); e < end * chunks; e += kStoreThreads) {
-                const int r = e / chunks, d0 = (e - r * chunks) * 16;
+            const int chunks = hdp / 16, shift = __ffs(chunks) - 1;
+            for (int e = tid + (grew ? 0 : off << shift); e < end << shift; e += blockDim.x) {
+                const int r = e >> shift, d0 = (e - (r << shift)) * 16;
                 if (d0 >= hd) continue; // padding: stays zero
                 uint4 *dst = reinterpret_cast<uint4 *>(page + (size_t)(r >> 4) * 16 * hdp +
                                                        kv_key_offset(hdp, r & 15, d0));
-                unsigned w[4] = {0, 0, 0, 0};
+                uint4 w;
                 if (r < off) {
                     const uint4 o = *dst;
-                    const unsigned ow[4] = {o.x, o.y, o.z, o.w};
-#pragma unroll
-                    for (int u = 0; u < 16; u++)
-                        w[u >> 2] |= ((unsigned)recode((int)(int8_t)byte_of(ow[u >> 2], u & 3), was, now, ratio) & 0xffu)
-                                     << (8 * (u & 3));
+                    w = make_uint4(recode4(o.x, was, now, ratio), recode4(o.y, was, now, ratio),
+                                   recode4(o.z, was, now, ratio), recode4(o.w, was, now, ratio));
                 } else {
                     const T *x = xs + (r - off) * hd + d0;
 #pragma unroll
-                    for (int u = 0; u < 16; u++)
-                        if (d0 + u < hd) w[u >> 2] |= ((unsigned)code_of(to_f(x[u]), now, inv) & 0xffu) << (8 * (u & 3));
+                    for (int q = 0; q < 4; q += 2) {
+                        float y[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+                        if (d0 + 4 * q < hd) eight_at(x + 4 * q, y);
+                        (&w.x)[q] = codes4({y[0], y[1], y[2], y[3]}, now, inv, easy);
+                        (&w.x)[q + 1] = codes4({y[4], y[5], y[6], y[7]}, now, inv, easy);
+                    }
                 }
-                *dst = make_uint4(w[0], w[1], w[2], w[3]);
+                *dst = w;
             }
         } else {
+            // a thread: two dimensions of a block, so that a token's pair is one read
             const int b0 = grew ? 0 : off >> 4, nb = ((end + 15) >> 4) - b0;
-            for (int e = tid; e < nb * hd; e += kStoreThreads) {
-                const int b = e / hd, d = e - b * hd, r0 = (b0 + b) << 4;
-                uint4 *dst = reinterpret_cast<uint4 *>(page + (size_t)(b0 + b) * 16 * hdp + d * 16);
-                unsigned w[4] = {0, 0, 0, 0};
-                if (r0 < off || r0 + 16 > end) {
-                    const uint4 o = *dst;
-                    w[0] = o.x, w[1] = o.y, w[2] = o.z, w[3] = o.w;
-                }
+            Places at(hd / 2);
+            for (int e = tid; e < nb * (hd / 2); e += blockDim.x, at.step()) {
+                const int d = 2 * at.r, r0 = (b0 + at.q) << 4;
+                uint4 *dst = reinterpret_cast<uint4 *>(page + (size_t)(b0 + at.q) * 16 * hdp + d * 16);
+                uint4 w[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+                const bool all = r0 >= off && r0 + 16 <= end; // else some positions stay, or are rounded again
+                if (!all) w[0] = dst[0], w[1] = dst[1];
 #pragma unroll
-                for (int u = 0; u < 16; u++) {
-                    const int r = r0 + u, sh = 8 * (u & 3);
-                    unsigned q;
-                    if (r >= off && r < end)
-                        q = (unsigned)code_of(to_f(xs[(r - off) * hd + d]), now, inv);
-                    else if (r < off && grew)
-                        q = (unsigned)recode((int)(int8_t)byte_of(w[u >> 2], u & 3), was, now, ratio);
-                    else
-                        continue;
-                    w[u >> 2] = (w[u >> 2] & ~(0xffu << sh)) | ((q & 0xffu) << sh);
+                for (int q = 0; q < 4; q++) {
+                    const int r = r0 + 4 * q - off; // first of four tokens, in the run
+                    if (!all && grew && r < 0) { // positions before the run
+                        const unsigned old = r + 3 < 0 ? 0xffffffffu : 0xffffffffu >> 8 * (r + 4);
+#pragma unroll
+                        for (int h = 0; h < 2; h++) {
+                            unsigned &o = (&w[h].x)[q];
+                            o = (o & ~old) | (recode4(o, was, now, ratio) & old);
+                        }
+                    }
+                    if (!all && (r + 3 < 0 || r >= run)) continue;
+                    float y[2][4];
+                    unsigned keep = 0;
+#pragma unroll
+                    for (int u = 0; u < 4; u++) {
+                        const bool fresh = all || (r + u >= 0 && r + u < run);
+                        const float2 z = fresh ? pair_at(xs + (r + u) * hd + d) : make_float2(0.f, 0.f);
+                        y[0][u] = z.x, y[1][u] = z.y;
+                        if (!fresh) keep |= 0xffu << 8 * u;
+                    }
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        unsigned &o = (&w[h].x)[q];
+                        o = (o & keep) | (codes4(y[h], now, inv, easy) & ~keep);
+                    }
                 }
-                *dst = make_uint4(w[0], w[1], w[2], w[3]);
+                dst[0] = w[0], dst[1] = w[1];
             }
         }
-        __syncthreads(); // every thread has read the scale and the staged run
         if (tid == 0) *place = now;
+        __syncthreads(); // the staged run is read
     }
 }
 
@@ -218,18 +290,20 @@ struct WriteCodes {
     }
 };
 
-// Codes of a page and head to W at [row][n_kv][hd] element offsets from `to`.
+// Codes of a page and head to W at [row][n_kv][hd] element offsets from `to`; keys (side 0) or values.
 template <class W>
-__device__ __forceinline__ void page_out(const TqKvView &c, int id, int head, size_t to, const W &wk, const W &wv) {
+__device__ __forceinline__ void page_out(const TqKvView &c, int id, int head, size_t to, const W &wk, const W &wv,
+                                         int side) {
     const int hd = c.hd, hdp = c.hdp, q = hd / 4, row = c.n_kv * hd;
     const int8_t *pk = c.k + kv_block_offset(c, id, head, 0), *pv = c.v + kv_block_offset(c, id, head, 0);
-    for (int e = threadIdx.x; e < c.page * q; e += blockDim.x) {
+#pragma unroll 4
+    for (int e = threadIdx.x; side == 0 && e < c.page * q; e += blockDim.x) {
         const int r = e / q, d = (e - r * q) * 4;
         const unsigned w =
             *reinterpret_cast<const unsigned *>(pk + (size_t)(r >> 4) * 16 * hdp + kv_key_offset(hdp, r & 15, d));
         wk(to + (size_t)r * row + d, w);
     }
-    for (int e = threadIdx.x; e < (c.page >> 4) * q; e += blockDim.x) {
+    for (int e = threadIdx.x; side == 1 && e < (c.page >> 4) * q; e += blockDim.x) {
         const int b = e / q, d = (e - b * q) * 4;
         const uint4 *p = reinterpret_cast<const uint4 *>(pv + (size_t)b * 16 * hdp + d * 16);
         const uint4 x[4] = {p[0], p[1], p[2], p[3]};
@@ -249,7 +323,7 @@ __global__ void kv_read_kernel(TqKvView c, const int *pages, float *k, float *v)
     if (!page_of(c, pages, blockIdx.x, &id)) return;
     const float2 s = c.scale[(size_t)id * c.n_kv + blockIdx.y];
     const size_t to = ((size_t)blockIdx.x * c.page * c.n_kv + blockIdx.y) * c.hd;
-    page_out(c, id, blockIdx.y, to, WriteValues{k, s.x}, WriteValues{v, s.y});
+    page_out(c, id, blockIdx.y, to, WriteValues{k, s.x}, WriteValues{v, s.y}, blockIdx.z);
 }
 
 __global__ void kv_save_kernel(TqKvView c, const int *pages, int8_t *k, int8_t *v, float *ks, float *vs) {
@@ -257,8 +331,8 @@ __global__ void kv_save_kernel(TqKvView c, const int *pages, int8_t *k, int8_t *
     if (!page_of(c, pages, blockIdx.x, &id)) return;
     const float2 s = c.scale[(size_t)id * c.n_kv + blockIdx.y];
     const size_t to = ((size_t)blockIdx.x * c.page * c.n_kv + blockIdx.y) * c.hd;
-    page_out(c, id, blockIdx.y, to, WriteCodes{k, 0.f}, WriteCodes{v, 0.f});
-    if (threadIdx.x == 0) {
+    page_out(c, id, blockIdx.y, to, WriteCodes{k, 0.f}, WriteCodes{v, 0.f}, blockIdx.z);
+    if (threadIdx.x == 0 && blockIdx.z == 0) {
         ks[(size_t)blockIdx.x * c.n_kv + blockIdx.y] = s.x;
         vs[(size_t)blockIdx.x * c.n_kv + blockIdx.y] = s.y;
     }
@@ -322,14 +396,15 @@ cudaError_t launch_store(const TqKvView &c, const T *k, const T *v, long long ks
     if (e != cudaSuccess) return e;
     // A decode step's tokens are runs of one: a block each. In a prompt most
     // tokens are not the first of their page, so a block looks through several.
-    const int window = n <= 1024 ? 1 : TQ_KV_BLOCK;
+    const int window = n <= 1024 ? 1 : c.page >= 32 ? 32 : 16;
+    const int threads = c.page * c.hd <= 4096 || n <= 1024 ? kStoreThreads / 2 : kStoreThreads;
     const dim3 grid((n + window - 1) / window, c.n_kv, 2);
     const size_t ax = (uintptr_t)k | (uintptr_t)v | (size_t)(ks * (long long)sizeof(T)) |
                       (size_t)(vs * (long long)sizeof(T)) | (size_t)c.hd * sizeof(T);
     if (ax % 16 == 0)
-        kv_store_kernel<T, true><<<grid, kStoreThreads, smem, st>>>(c, k, v, ks, vs, slots, n, window);
+        kv_store_kernel<T, true><<<grid, threads, smem, st>>>(c, k, v, ks, vs, slots, n, window);
     else
-        kv_store_kernel<T, false><<<grid, kStoreThreads, smem, st>>>(c, k, v, ks, vs, slots, n, window);
+        kv_store_kernel<T, false><<<grid, threads, smem, st>>>(c, k, v, ks, vs, slots, n, window);
     return cudaGetLastError();
 }
 
@@ -355,12 +430,12 @@ cudaError_t tq_kv_launch_load(const TqKvView &v, const int *pages, int n, const 
 cudaError_t tq_kv_launch_save(const TqKvView &v, const int *pages, int n, int8_t *k, int8_t *val, float *kscale,
                               float *vscale, cudaStream_t st) {
     if (n == 0) return cudaSuccess;
-    kv_save_kernel<<<dim3(n, v.n_kv), kPageThreads, 0, st>>>(v, pages, k, val, kscale, vscale);
+    kv_save_kernel<<<dim3(n, v.n_kv, 2), kPageThreads, 0, st>>>(v, pages, k, val, kscale, vscale);
     return cudaGetLastError();
 }
 
 cudaError_t tq_kv_launch_read(const TqKvView &v, const int *pages, int n, float *k, float *val, cudaStream_t st) {
     if (n == 0) return cudaSuccess;
-    kv_read_kernel<<<dim3(n, v.n_kv), kPageThreads, 0, st>>>(v, pages, k, val);
+    kv_read_kernel<<<dim3(n, v.n_kv, 2), kPageThreads, 0, st>>>(v, pages, k, val);
     return cudaGetLastError();
 }
