@@ -369,6 +369,18 @@ TQ_EXPORT int tq_qwen_load_tensor(uint64_t model, const char *name, const void *
  * memory. */
 TQ_EXPORT int tq_qwen_set_prefill(uint64_t model, int rows);
 
+/* What tq_qwen_generate keeps its keys and values in. TQ_CACHE_F32 (the
+ * default): float32, as the reference does, the parity mode. TQ_CACHE_INT8: the
+ * paged 8-bit cache below (tq_kv_*, pages of 64 positions, a scale for each page
+ * and KV head), a quarter of the memory and of the bytes that a step's attention
+ * reads; the prompt and the steps run tq_kv_plan_dev, tq_kv_store_dev and
+ * tq_kv_attention_dev, and the generated ids may differ from the parity mode's.
+ * The other cache's memory is released. Every rank of a tensor-parallel model
+ * calls it alike. */
+#define TQ_CACHE_F32 0
+#define TQ_CACHE_INT8 1
+TQ_EXPORT int tq_qwen_set_cache(uint64_t model, int kind);
+
 /* tq_gpt2_set_sampling for a Qwen2 model (main.go:115-150); one GPU only
  * (TQ_ERR_UNSUPPORTED when world > 1: the lm head is split by vocabulary).
  * During a token-by-token prompt every step runs the sample step too (its

@@ -50,6 +50,7 @@
 #define TQ_DECODE_PDL 0
 #include "tq_decode.cuh"
 #include "tq_internal.h"
+#include "tq_kv.h"
 #include "tq_ptx.cuh"
 
 namespace {
@@ -264,6 +265,39 @@ __global__ void rope_rows_kernel(float *qkv, int qkvc, int nq, int nkv, int hd, 
         kd[j + half] = r1;
     }
     for (int j = threadIdx.x; j < kvd; j += blockDim.x) vd[j] = __fadd_rn(v[j], vbias[j]);
+}
+
+// Rows of a fused q|k|v for the 8-bit cache (tq_qwen_set_cache): the biases
+// added, q and k rotated, all in place; row r is at position pos0 + r, or, with a
+// state, at the state's. cs: the step's table, or null to make the row's own.
+// A block a row and head (query heads, then KV heads with their values).
+__global__ void rope_inplace_kernel(float *qkv, int qkvc, int nq, int nkv, int hd, int pos0, const int *state,
+                                    const double *cs, double theta, const float *bias) {
+    step_entry();
+    __shared__ double own[kAttMaxHd];
+    const int r = blockIdx.y, h = blockIdx.x, half = hd / 2;
+    if (!cs) {
+        rope_table(own, state ? state[1] : pos0 + r, hd, theta);
+        __syncthreads();
+        cs = own;
+    }
+    float *x = qkv + (size_t)r * qkvc + h * hd;
+    const float *b = bias + h * hd;
+    for (int i = threadIdx.x; i < half; i += blockDim.x) {
+        float r0, r1;
+        rope_pair(cs, i, __fadd_rn(x[i], b[i]), __fadd_rn(x[i + half], b[i + half]), r0, r1);
+        x[i] = r0;
+        x[i + half] = r1;
+    }
+    if (h < nq) return;
+    x += nkv * hd, b += nkv * hd;
+    for (int i = threadIdx.x; i < hd; i += blockDim.x) x[i] = __fadd_rn(x[i], b[i]);
+}
+
+// The lengths of a prompt chunk for the cache's plan: held = pos, added = rows.
+__global__ void kv_chunk_kernel(int *held, int *added, int pos, int rows) {
+    *held = pos;
+    *added = rows;
 }
 
 // Causal attention of a prompt chunk's rows (model.go:262-293 per row):
@@ -684,6 +718,13 @@ struct Qwen {
     ArLink ar{};
     unsigned long long *ar_area = nullptr; // this rank's slot area (exported by IPC)
     size_t ar_smem = 0;                    // ar_rmsnorm_kernel's dynamic shared memory
+    // tq_qwen_set_cache: the 8-bit cache in place of the layers' kc / vc
+    uint64_t kv = 0;
+    int *kv_ints = nullptr; // starts [2], lens, added, chunk held, chunk added, free count, then the table and free pages
+    long long *kv_slots = nullptr;
+    void *kv_space = nullptr;
+    size_t kv_space_bytes = 0;
+    int kv_pages = 0, kv_slots_cap = 0;
     // tq_qwen_set_sampling (one GPU): temp > 0 draws generated token k with draws[k]
     double temp = 0;
     double *draws = nullptr;
@@ -724,6 +765,8 @@ void destroy(Qwen &m) {
     m.ar_on = false;
     if (m.comm) g_nccl.commDestroy(m.comm);
     m.comm = nullptr;
+    tq_kv_free(m.kv);
+    m.kv = 0;
     for (Layer &l : m.L) {
         for (TqMatrixDev *w : {&l.qkv, &l.o, &l.gu, &l.down}) tq_release_matrix(w);
         for (void *p : {l.stage_qkv, l.stage_gu})
@@ -965,6 +1008,71 @@ cudaError_t ar_setup(Qwen &m) {
     return cudaSuccess;
 }
 
+// ---- the 8-bit cache (tq_qwen_set_cache) ----------------------------------------
+constexpr int kKvPage = 64;
+enum { kKvStarts = 0, kKvLens = 2, kKvOne = 3, kKvHeld = 4, kKvAdded = 5, kKvFree = 6, kKvTable = 8 };
+
+cudaError_t kv_call(int rc) { return rc == TQ_OK ? cudaSuccess : rc == TQ_ERR_NOMEM ? cudaErrorMemoryAllocation : cudaErrorUnknown; }
+
+// Frees a buffer that dalloc made.
+void dfree(Qwen &m, void *p) {
+    for (size_t i = 0; i < m.allocs.size(); i++)
+        if (m.allocs[i] == p) {
+            cudaFree(p);
+            m.allocs.erase(m.allocs.begin() + i);
+            return;
+        }
+}
+
+// A new sequence: all pages free, in order.
+cudaError_t kv_reset(Qwen &m) {
+    if (!m.kv) return cudaSuccess;
+    return cudaMemcpyAsync(m.kv_ints + kKvFree, &m.kv_pages, sizeof(int), cudaMemcpyHostToDevice, m.st);
+}
+
+// Pages and slots of the next tokens: `held` positions before, `added` of them.
+cudaError_t kv_plan(Qwen &m, const int *held, const int *added) {
+    tq_kv_plan_args a{};
+    a.n = 1;
+    a.table_stride = a.table_cols = a.free_cap = m.kv_pages;
+    a.slots_cap = m.kv_slots_cap;
+    a.cached = held;
+    a.added = added;
+    a.table = m.kv_ints + kKvTable;
+    a.free_pages = a.table + m.kv_pages;
+    a.free_count = a.free_left = m.kv_ints + kKvFree;
+    a.starts = m.kv_ints + kKvStarts;
+    a.lens = m.kv_ints + kKvLens;
+    a.slots = m.kv_slots;
+    return kv_call(tq_kv_plan_dev(m.kv, &a, m.st));
+}
+
+// RoPE of `rows` fused q|k|v rows, their keys and values into layer l of the
+// cache, and the rows' attention over it.
+cudaError_t kv_attention(Qwen &m, int l, float *qkv, int rows, float *out, int pos0, const int *state, const double *cs) {
+    const int qkvc = m.qd + 2 * m.kvd;
+    TRY(step_launch(rope_inplace_kernel, dim3(m.nq + m.nkv, rows), dim3(m.hd <= 128 ? 64 : 128), 0, m.st, qkv, qkvc,
+                    m.nq, m.nkv, m.hd, pos0, state, cs, m.c.theta, m.L[l].qkvb));
+    TRY(kv_call(tq_kv_store_dev(m.kv, l, qkv + m.qd, qkv + m.qd + m.kvd, TQ_LINEAR_F32, qkvc, qkvc, m.kv_slots, rows, m.st)));
+    tq_kv_attention_args a{};
+    a.q = qkv;
+    a.out = out;
+    a.dtype = TQ_LINEAR_F32;
+    a.n_q = m.nq;
+    a.n_tokens = rows;
+    a.n = 1;
+    a.q_stride = qkvc;
+    a.out_stride = m.qd;
+    a.starts = m.kv_ints + kKvStarts;
+    a.lens = m.kv_ints + kKvLens;
+    a.table = m.kv_ints + kKvTable;
+    a.table_stride = a.table_cols = m.kv_pages;
+    a.scale = (float)(1.0 / sqrt((double)m.hd));
+    a.workspace = m.kv_space;
+    a.workspace_bytes = m.kv_space_bytes;
+    return kv_call(tq_kv_attention_dev(m.kv, l, &a, m.st));
+}
+
 // One step (model.go:232-307) for the state's token at the state's position.
 // The gate|up matvec ends with SiLU(gate) * up; the attention's scores pass
 // applies RoPE and fills the caches. A residual add and the RMSNorm after it
@@ -991,6 +1099,7 @@ cudaError_t step(Qwen &m, int n_prompt) {
         // 512 threads: small enough to be resident beside the matvec before it, ready when it completes
         return step_launch_early(rmsnorm_kernel, dim3(1), dim3(512), 0, m.st, m.x, m.y, w, m.a, d, m.c.eps);
     };
+    if (m.kv) TRY(kv_plan(m, m.state + 1, m.kv_ints + kKvOne));
     bool pending = false; // the previous down_proj output is still to be added to x
     for (Layer &ly : m.L) {
         if (pending) TRY(add_norm(ly.ln1));
@@ -1000,8 +1109,11 @@ cudaError_t step(Qwen &m, int n_prompt) {
         rope.vbias = ly.qkvb + m.qd + m.kvd;
         rope.kc = ly.kc;
         rope.vc = ly.vc;
-        TRY(decode_attention(m.qkv, ly.kc, ly.vc, m.kvd, m.att, m.state, m.nq, m.hd, m.group,
-                             1.0 / sqrt((double)m.hd), m.att_scr, m.st, rope, m.world == 1));
+        if (m.kv)
+            TRY(kv_attention(m, (int)(&ly - m.L.data()), m.qkv, 1, m.att, 0, m.state, m.rope));
+        else
+            TRY(decode_attention(m.qkv, ly.kc, ly.vc, m.kvd, m.att, m.state, m.nq, m.hd, m.group,
+                                 1.0 / sqrt((double)m.hd), m.att_scr, m.st, rope, m.world == 1));
         TRY(tq_launch_matmul(ly.o, m.att + m.arow, m.y, 1, m.scr, m.st));
         TRY(add_norm(ly.ln2)); // x += o_proj, then norm
         TRY(tq_launch_cmv_epi(ly.gu, m.a, m.h, m.scr, m.st, TQ_EPI_SWIGLU, tq_matvec_uses_tmv()));
@@ -1040,6 +1152,11 @@ cudaError_t prefill(Qwen &m, int n_prompt) {
         const int rows = n_prompt - c0 < R ? n_prompt - c0 : R;
         embed_rows_kernel<<<rows, 1024, 0, m.st>>>(m.embed, m.prompt, c0, m.px, m.L[0].ln1, m.pa, d, m.c.eps);
         TRY(cudaGetLastError());
+        if (m.kv) {
+            kv_chunk_kernel<<<1, 1, 0, m.st>>>(m.kv_ints + kKvHeld, m.kv_ints + kKvAdded, c0, rows);
+            TRY(cudaGetLastError());
+            TRY(kv_plan(m, m.kv_ints + kKvHeld, m.kv_ints + kKvAdded));
+        }
         for (size_t l = 0; l < m.L.size(); l++) {
             Layer &ly = m.L[l];
             if (l > 0) { // x += the previous layer's down_proj, then the norm
@@ -1047,11 +1164,15 @@ cudaError_t prefill(Qwen &m, int n_prompt) {
                 TRY(cudaGetLastError());
             }
             TRY(tq_launch_matmul(ly.qkv, m.pa, m.pqkv, rows, m.scr, m.st));
-            rope_rows_kernel<<<rows, 256, 0, m.st>>>(m.pqkv, qkvc, m.nq, m.nkv, m.hd, c0, m.c.theta, ly.qkvb,
-                                                     ly.qkvb + m.qd, ly.qkvb + m.qd + m.kvd, ly.kc, ly.vc);
-            prefill_attention_kernel<<<dim3(m.nq, (rows + kPfRows - 1) / kPfRows), kPfThreads, pf_smem, m.st>>>(
-                m.pqkv, qkvc, ly.kc, ly.vc, m.kvd, m.patt, m.qd, m.hd, m.group, scale, c0, rows, n_prompt);
-            TRY(cudaGetLastError());
+            if (m.kv) {
+                TRY(kv_attention(m, (int)l, m.pqkv, rows, m.patt, c0, nullptr, nullptr));
+            } else {
+                rope_rows_kernel<<<rows, 256, 0, m.st>>>(m.pqkv, qkvc, m.nq, m.nkv, m.hd, c0, m.c.theta, ly.qkvb,
+                                                         ly.qkvb + m.qd, ly.qkvb + m.qd + m.kvd, ly.kc, ly.vc);
+                prefill_attention_kernel<<<dim3(m.nq, (rows + kPfRows - 1) / kPfRows), kPfThreads, pf_smem, m.st>>>(
+                    m.pqkv, qkvc, ly.kc, ly.vc, m.kvd, m.patt, m.qd, m.hd, m.group, scale, c0, rows, n_prompt);
+                TRY(cudaGetLastError());
+            }
             TRY(tq_launch_matmul(ly.o, m.patt, m.py, rows, m.scr, m.st));
             if (m.world > 1)
                 TRY(nccl_err(g_nccl.allReduce(m.py, m.py, (size_t)rows * d, ncclFloat32, ncclSum, m.comm, m.st)));
@@ -1317,6 +1438,7 @@ int tq_qwen_generate(uint64_t model, const int *prompt, int n_prompt, int n_gen,
         if (e == cudaSuccess) m->prompt_cap = n_prompt;
     }
     if (e == cudaSuccess) e = cudaMemcpyAsync(m->prompt, prompt, sizeof(int) * n_prompt, cudaMemcpyHostToDevice, m->st);
+    if (e == cudaSuccess) e = kv_reset(*m);
     cudaEvent_t ev[3] = {};
     for (int i = 0; i < 3 && e == cudaSuccess; i++) e = cudaEventCreate(&ev[i]);
     if (e == cudaSuccess) {
@@ -1332,6 +1454,7 @@ int tq_qwen_generate(uint64_t model, const int *prompt, int n_prompt, int n_gen,
         e = step(*m, n_prompt); // eager first step: kernel set-up outside the capture
         if (e == cudaSuccess) e = cudaStreamSynchronize(m->st);
         set_state_kernel<<<1, 1, 0, m->st>>>(m->state, prompt[0], 0, 0); // start the sequence over
+        if (e == cudaSuccess) e = kv_reset(*m);
         cudaGraph_t g = nullptr;
         if (e == cudaSuccess) e = cudaStreamBeginCapture(m->st, cudaStreamCaptureModeThreadLocal);
         if (e == cudaSuccess) {
@@ -1364,6 +1487,72 @@ int tq_qwen_generate(uint64_t model, const int *prompt, int n_prompt, int n_gen,
     unsigned status = 0;
     if ((e = tq_read_status(m->scr, m->st, &status)) != cudaSuccess) return tq_cuda_fail(e, "status read");
     if (status & TQ_STATUS_TIMEOUT) return tq_fail(TQ_ERR_TIMEOUT, "tensai: a kernel timed out during decode");
+    if (m->kv) {
+        unsigned bits = 0;
+        if ((rc = tq_kv_status(m->kv, &bits)) != TQ_OK) return rc;
+        if (bits & TQ_KV_STATUS_TIMEOUT) return tq_fail(TQ_ERR_TIMEOUT, "tensai: a kernel timed out during decode");
+        if (bits) return tq_fail(TQ_ERR_CUDA, "tensai: the 8-bit cache reports status %u", bits);
+    }
+    return TQ_OK;
+}
+
+int tq_qwen_set_cache(uint64_t model, int kind) {
+    int rc = TQ_OK;
+    auto m = find(model, &rc);
+    if (!m) return rc;
+    if (kind != TQ_CACHE_F32 && kind != TQ_CACHE_INT8)
+        return tq_fail(TQ_ERR_ARG, "tensai: cache kind must be %d or %d, got %d", TQ_CACHE_F32, TQ_CACHE_INT8, kind);
+    if ((kind == TQ_CACHE_INT8) == (m->kv != 0)) return TQ_OK;
+    cudaError_t e = cudaSetDevice(m->device);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(m->st);
+    if (e != cudaSuccess) return tq_cuda_fail(e, "cache set-up");
+    if (m->graph) cudaGraphExecDestroy(m->graph); // the graph holds the previous cache
+    m->graph = nullptr;
+    auto drop_kv = [&]() {
+        tq_kv_free(m->kv);
+        m->kv = 0;
+        dfree(*m, m->kv_ints), dfree(*m, m->kv_slots), dfree(*m, m->kv_space);
+        m->kv_ints = nullptr, m->kv_slots = nullptr, m->kv_space = nullptr;
+    };
+    if (kind == TQ_CACHE_F32) { // the float32 caches first: on failure the 8-bit one stays
+        const size_t bytes = sizeof(float) * (size_t)m->c.ctx * m->kvd;
+        for (Layer &ly : m->L)
+            for (float **p : {&ly.kc, &ly.vc})
+                if (e == cudaSuccess && !*p) e = dalloc(*m, (void **)p, bytes);
+        if (e != cudaSuccess) {
+            for (Layer &ly : m->L)
+                for (float **p : {&ly.kc, &ly.vc}) dfree(*m, *p), *p = nullptr;
+            return tq_cuda_fail(e, "float32 cache allocation");
+        }
+        drop_kv();
+        return TQ_OK;
+    }
+    m->kv_pages = (m->c.ctx + kKvPage - 1) / kKvPage;
+    m->kv_slots_cap = TQ_MM_MAX_ROWS;
+    const tq_kv_config cfg = {m->c.n_layer, m->nkv, m->hd, kKvPage, m->kv_pages};
+    uint64_t kv = 0;
+    if ((rc = tq_kv_create(&cfg, &kv)) != TQ_OK) return rc;
+    m->kv = kv;
+    std::vector<int> ints(kKvTable + 2 * (size_t)m->kv_pages, 0);
+    ints[kKvOne] = 1;
+    ints[kKvFree] = m->kv_pages;
+    for (int i = 0; i < m->kv_pages; i++) ints[kKvTable + m->kv_pages + i] = m->kv_pages - 1 - i; // page 0 on top
+    rc = tq_kv_attention_workspace(kv, &m->kv_space_bytes);
+    if (rc == TQ_OK) {
+        e = dalloc(*m, (void **)&m->kv_ints, sizeof(int) * ints.size());
+        if (e == cudaSuccess) e = dalloc(*m, (void **)&m->kv_slots, sizeof(long long) * m->kv_slots_cap);
+        if (e == cudaSuccess) e = dalloc(*m, &m->kv_space, m->kv_space_bytes);
+        if (e == cudaSuccess) e = cudaMemset(m->kv_space, 0, TQ_KV_WORKSPACE_HEAD);
+        if (e == cudaSuccess)
+            e = cudaMemcpy(m->kv_ints, ints.data(), sizeof(int) * ints.size(), cudaMemcpyHostToDevice);
+        if (e == cudaSuccess) e = cudaDeviceSynchronize();
+    }
+    if (rc != TQ_OK || e != cudaSuccess) {
+        drop_kv();
+        return rc != TQ_OK ? rc : tq_cuda_fail(e, "8-bit cache set-up");
+    }
+    for (Layer &ly : m->L)
+        for (float **p : {&ly.kc, &ly.vc}) dfree(*m, *p), *p = nullptr;
     return TQ_OK;
 }
 

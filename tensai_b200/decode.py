@@ -245,6 +245,14 @@ class Qwen:
         tensor-core matmul (tq_qwen_set_prefill)."""
         _lib.check(_lib.load().tq_qwen_set_prefill(self.handle, rows))
 
+    def set_cache(self, kind: str) -> None:
+        """"float32" (the reference's way, the parity mode) or "int8": the paged
+        8-bit cache, a quarter of the memory (tq_qwen_set_cache)."""
+        kinds = {"float32": _lib.TQ_CACHE_F32, "int8": _lib.TQ_CACHE_INT8}
+        if kind not in kinds:
+            raise ValueError(f'tensai: cache must be "float32" or "int8", got {kind!r}')
+        _lib.check(_lib.load().tq_qwen_set_cache(self.handle, kinds[kind]))
+
     def set_sampling(self, temp: float, draws=None) -> None:
         """As Gpt2.set_sampling (tq_qwen_set_sampling; one GPU only)."""
         d = np.ascontiguousarray(draws if draws is not None else [], np.float64)
