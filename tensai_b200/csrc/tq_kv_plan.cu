@@ -12,8 +12,8 @@
 //
 // One launch of one cluster of 1 to 8 blocks: the blocks share the entries and
 // slots evenly, and the cluster's barrier separates all reads of the lengths
-// and the free count from their updates in place, so a graph that holds the
-// step can be replayed without a copy of either. Bound by latency: the launch,
+// (into every block's shared memory) and the free count from their updates in
+// place, so a graph that holds the step can be replayed without a copy of either. Bound by latency: the launch,
 // two dependent loads, two scans.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
@@ -29,18 +29,19 @@ namespace cg = cooperative_groups;
 
 constexpr int kThreads = 1024;
 constexpr int kMaxCluster = 8;
+constexpr int kSide = 4; // slots that a thread finds side by side
 
-// The largest i < n with sums[i] <= x, for ascending sums[0] = 0 .. sums[n] > x.
-__device__ __forceinline__ int find_row(const int *sums, int n, int x) {
-    int lo = 0, hi = n;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (sums[mid] <= x)
-            lo = mid;
-        else
-            hi = mid;
-    }
-    return lo;
+// For each of B values x: the largest i < n with sums[i] <= x, for ascending
+// sums[0] = 0 .. sums[n] > x; the B searches run side by side.
+template <int B> __device__ __forceinline__ void find_rows(const int *sums, int n, const int (&x)[B], int (&row)[B]) {
+#pragma unroll
+    for (int u = 0; u < B; u++) row[u] = 0;
+    for (int step = 1 << (31 - __clz(n)); step; step >>= 1)
+#pragma unroll
+        for (int u = 0; u < B; u++) {
+            const int at = row[u] + step;
+            if (at < n && sums[at] <= x[u]) row[u] = at;
+        }
 }
 
 // The or of every thread's bits, to all of them. *sh: zero before a barrier that precedes the call.
@@ -78,22 +79,23 @@ __device__ __forceinline__ void block_scan(long long &a, long long &b, long long
 }
 
 __global__ void __launch_bounds__(kThreads) kv_plan_kernel(tq_kv_plan_args a, int shift, int n_pages, unsigned *status) {
-    extern __shared__ int sums[]; // [n + 1] token starts, [n + 1] new-page starts
-    int *tok = sums, *pag = sums + a.n + 1;
+    extern __shared__ int sums[]; // [n + 1] token starts, [n + 1] new-page starts, [n] cached
+    int *tok = sums, *pag = sums + a.n + 1, *held = pag + a.n + 1;
+    __shared__ unsigned s_bad;
     const int n = a.n, tid = threadIdx.x, P = 1 << shift;
     cg::cluster_group cl = cg::this_cluster();
     const int rank = (int)cl.block_rank(), blocks = (int)cl.num_blocks();
     const int per = (n + kThreads - 1) / kThreads, i0 = min(n, tid * per), i1 = min(n, i0 + per);
     const int count = *a.free_count;
-    long long st = 0, sp = 0;
-    __shared__ unsigned s_bad;
     if (tid == 0) s_bad = 0;
+    long long st = 0, sp = 0;
     unsigned bad = 0;
     for (int i = i0; i < i1; i++) {
-        const long long c = a.cached[i], d = a.added[i];
-        if (c < 0 || d < 0) bad |= TQ_KV_STATUS_LENGTH;
-        const long long have = (c + P - 1) >> shift, want = (c + d + P - 1) >> shift;
-        if (c + d > INT_MAX) bad |= TQ_KV_STATUS_LENGTH;
+        const int ci = a.cached[i], di = a.added[i];
+        held[i] = ci;
+        tok[i] = di; // until the sums are known
+        const long long c = ci, d = di, have = (c + P - 1) >> shift, want = (c + d + P - 1) >> shift;
+        if (c < 0 || d < 0 || c + d > INT_MAX) bad |= TQ_KV_STATUS_LENGTH;
         if (want > a.table_cols) bad |= TQ_KV_STATUS_TABLE;
         st += d;
         sp += want - have;
@@ -104,19 +106,19 @@ __global__ void __launch_bounds__(kThreads) kv_plan_kernel(tq_kv_plan_args a, in
     if (count < 0 || count > a.free_cap) bad |= TQ_KV_STATUS_LENGTH;
     if (pages > count) bad |= TQ_KV_STATUS_POOL;
     bad = block_or(bad, &s_bad); // one verdict for the block; every block of the cluster reaches the same one
+    if (blocks > 1) cl.barrier_arrive(); // this block has read what may be written in place
+    const int g = rank * kThreads + tid, stride = blocks * kThreads;
     if (bad) {
-        if (rank == 0 && tid == 0) atomicOr(status, bad);
-        cl.sync();
-        const int g = rank * kThreads + tid, stride = blocks * kThreads;
+        if (g == 0) atomicOr(status, bad);
         for (int i = g; i <= n; i += stride) a.starts[i] = 0;
-        if (a.lens != a.cached)
-            for (int i = g; i < n; i += stride) a.lens[i] = a.cached[i];
         for (int t = g; t < a.slots_cap; t += stride) a.slots[t] = -1;
+        if (blocks > 1) cl.barrier_wait();
+        for (int i = g; i < n; i += stride) a.lens[i] = held[i];
         if (g == 0) *a.free_left = count;
         return;
     }
     for (int i = i0; i < i1; i++) {
-        const int c = a.cached[i], d = a.added[i];
+        const int c = held[i], d = tok[i];
         tok[i] = (int)st;
         pag[i] = (int)sp;
         st += d;
@@ -124,36 +126,35 @@ __global__ void __launch_bounds__(kThreads) kv_plan_kernel(tq_kv_plan_args a, in
     }
     if (tid == 0) tok[n] = (int)tokens, pag[n] = (int)pages;
     __syncthreads();
-    const int g = rank * kThreads + tid, stride = blocks * kThreads;
-    for (int j = g; j < (int)pages; j += stride) { // new table entries
-        const int i = find_row(pag, n, j), id = a.free_pages[count - 1 - j];
-        if (id < 0 || id >= n_pages) atomicOr(status, TQ_KV_STATUS_PAGE);
-        a.table[(size_t)i * a.table_stride + ((a.cached[i] + P - 1) >> shift) + (j - pag[i])] = id;
-    }
-    for (int t = g; t < (int)tokens; t += stride) { // slots
-        const int i = find_row(tok, n, t), c = a.cached[i], pos = c + (t - tok[i]), have = (c + P - 1) >> shift;
-        const int b = pos >> shift;
-        const int id = b >= have ? a.free_pages[count - 1 - pag[i] - (b - have)] : a.table[(size_t)i * a.table_stride + b];
-        const bool ok = id >= 0 && id < n_pages;
-        if (!ok) atomicOr(status, TQ_KV_STATUS_PAGE);
-        a.slots[t] = ok ? ((long long)id << shift) + (pos & (P - 1)) : -1;
-    }
     for (int i = g; i <= n; i += stride) a.starts[i] = tok[i];
-    int keep[TQ_KV_MAX_REQUESTS / kThreads]; // lens may be cached: all of it is read before any is written
-    int held = 0;
-#pragma unroll
-    for (int u = 0; u < TQ_KV_MAX_REQUESTS / kThreads; u++) {
-        const int i = g + u * stride;
-        keep[u] = i < n ? a.cached[i] + (tok[i + 1] - tok[i]) : 0;
-        held += i < n;
+    for (int j0 = g; j0 < (int)pages; j0 += stride) { // new table entries
+        const int j[1] = {j0}, id = a.free_pages[count - 1 - j0];
+        int i[1];
+        find_rows(pag, n, j, i);
+        if (id < 0 || id >= n_pages) atomicOr(status, TQ_KV_STATUS_PAGE);
+        a.table[(size_t)i[0] * a.table_stride + ((held[i[0]] + P - 1) >> shift) + (j0 - pag[i[0]])] = id;
     }
-    if (blocks > 1)
-        cl.sync();
-    else
-        __syncthreads();
+    for (int t0 = g; t0 < (int)tokens; t0 += kSide * stride) { // slots
+        int t[kSide], i[kSide], pos[kSide], id[kSide];
 #pragma unroll
-    for (int u = 0; u < TQ_KV_MAX_REQUESTS / kThreads; u++)
-        if (u < held) a.lens[g + u * stride] = keep[u];
+        for (int u = 0; u < kSide; u++) t[u] = min(t0 + u * stride, (int)tokens - 1);
+        find_rows(tok, n, t, i);
+#pragma unroll
+        for (int u = 0; u < kSide; u++) {
+            const int c = held[i[u]], have = (c + P - 1) >> shift;
+            pos[u] = c + (t[u] - tok[i[u]]);
+            const int b = pos[u] >> shift;
+            id[u] = b >= have ? a.free_pages[count - 1 - pag[i[u]] - (b - have)] : a.table[(size_t)i[u] * a.table_stride + b];
+        }
+#pragma unroll
+        for (int u = 0; u < kSide; u++) {
+            const bool ok = id[u] >= 0 && id[u] < n_pages;
+            if (!ok) atomicOr(status, TQ_KV_STATUS_PAGE);
+            if (t0 + u * stride < (int)tokens) a.slots[t[u]] = ok ? ((long long)id[u] << shift) + (pos[u] & (P - 1)) : -1;
+        }
+    }
+    if (blocks > 1) cl.barrier_wait();
+    for (int i = g; i < n; i += stride) a.lens[i] = held[i] + (tok[i + 1] - tok[i]);
     if (g == 0) *a.free_left = count - (int)pages;
 }
 
@@ -192,7 +193,10 @@ __global__ void __launch_bounds__(kThreads) kv_release_kernel(tq_kv_release_args
     if (tid == 0) sums[n] = (int)pages;
     __syncthreads();
     for (int j = tid; j < (int)pages; j += kThreads) {
-        const int i = find_row(sums, n, j), id = a.table[(size_t)i * a.table_stride + (j - sums[i])];
+        const int x[1] = {j};
+        int i[1];
+        find_rows(sums, n, x, i);
+        const int id = a.table[(size_t)i[0] * a.table_stride + (j - sums[i[0]])];
         if (id < 0 || id >= n_pages) atomicOr(status, TQ_KV_STATUS_PAGE);
         a.free_pages[count + j] = id;
     }
@@ -208,10 +212,10 @@ cudaError_t set_up() {
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     return tq_device_once(g_once, dev, [] {
-        const int most = 2 * (TQ_KV_MAX_REQUESTS + 1) * (int)sizeof(int);
+        const int most = 3 * (TQ_KV_MAX_REQUESTS + 1) * (int)sizeof(int);
         cudaError_t r = cudaFuncSetAttribute(kv_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
         if (r == cudaSuccess)
-            r = cudaFuncSetAttribute(kv_release_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most / 2);
+            r = cudaFuncSetAttribute(kv_release_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most / 3);
         return r;
     });
 }
@@ -231,7 +235,7 @@ cudaError_t tq_kv_launch_plan(int page_shift, int n_pages, unsigned *status, con
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(blocks);
     cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = 2 * (size_t)(a.n + 1) * sizeof(int);
+    cfg.dynamicSmemBytes = 3 * (size_t)(a.n + 1) * sizeof(int);
     cfg.stream = st;
     cfg.attrs = attr;
     cfg.numAttrs = 1;

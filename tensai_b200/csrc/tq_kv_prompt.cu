@@ -46,8 +46,8 @@ constexpr int kConvThreads = 32 * kConvWarps;
 constexpr int kMmaWarp = kSoftWarps + kConvWarps; // one thread of it issues; the next warp loads
 constexpr int kThreads = 32 * (kMmaWarp + 2);
 constexpr int kConsts = 4;      // position tiles whose scales are kept
-constexpr int kSegCost = 3;     // what a segment costs besides its position tiles, in position tiles
-constexpr int kMinUnits = 5;    // units per CTA below which fewer CTAs work
+constexpr int kSegCost = 2;     // what a segment costs besides its position tiles, in position tiles
+constexpr int kMinUnits = 3;    // units per CTA below which fewer CTAs work
 constexpr float kSlack = 4.f;   // log2 by which w may exceed M
 constexpr float kUnit = 10.f;   // log2 of P at w = M
 constexpr float kLeast = 1e-30f; // least score factor of a block: -inf times it stays -inf

@@ -19,6 +19,7 @@ pool, a bad page id) is skipped there and raised by check().
 from __future__ import annotations
 
 import ctypes
+import struct
 
 from . import _lib
 from ._lib import TensaiError
@@ -29,6 +30,13 @@ _MESSAGES = ((_lib.TQ_KV_STATUS_POOL, "not enough free pages, or a full free lis
              (_lib.TQ_KV_STATUS_LENGTH, "a negative length or count, or starts that do not ascend"),
              (_lib.TQ_KV_STATUS_PAGE, "a page id or slot outside the cache"),
              (_lib.TQ_KV_STATUS_TIMEOUT, "a kernel gave up a bounded wait"))
+
+
+# The argument structs of include/tensai_cuda.h, packed: cheaper than a ctypes
+# Structure for each call of a decode step.
+_PLAN = struct.Struct("5i4x9Q").pack
+_RELEASE = struct.Struct("4i6Q").pack
+_ATTENTION = struct.Struct("2Q4i2q3Q2if4x2Q").pack
 
 
 def _refuse(msg: str):
@@ -53,6 +61,9 @@ class KVCache:
         dev = ctypes.c_int()
         _lib.check(self._L.tq_kv_info(self._h, None, ctypes.byref(dev)))
         self.device = torch.device("cuda", dev.value)
+        self._index = dev.value
+        self._i32, self._i64 = torch.int32, torch.int64
+        self._raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
         size = ctypes.c_size_t()
         _lib.check(self._L.tq_kv_attention_workspace(self._h, ctypes.byref(size)))
         self.workspace_bytes = size.value
@@ -63,32 +74,44 @@ class KVCache:
 
     # ---- arguments ----
     def _stream(self, stream) -> int:
-        return stream.cuda_stream if stream is not None else self._torch.cuda.current_stream(self.device).cuda_stream
+        if stream is not None:
+            return stream.cuda_stream
+        if self._raw_stream is not None:
+            return self._raw_stream(self._index)
+        return self._torch.cuda.current_stream(self.device).cuda_stream
 
     def _array(self, name, t, dtype, numel=None):
-        if t.dtype != dtype or t.device != self.device or not t.is_contiguous():
+        if t.dtype is not dtype or not t.is_cuda or t.get_device() != self._index or not t.is_contiguous():
             _refuse(f"{name}: a contiguous {dtype} tensor on {self.device} is required")
         if numel is not None and t.numel() != numel:
             _refuse(f"{name}: {t.numel()} elements, expected {numel}")
         return t.data_ptr()
 
     def _table(self, t, n):
-        if (t.dtype != self._torch.int32 or t.device != self.device or t.dim() != 2 or t.shape[0] != n
-                or (t.shape[1] > 1 and t.stride(1) != 1) or (n > 1 and t.stride(0) < t.shape[1])):
-            _refuse(f"table: an int32 tensor [{n}][pages of a request] on {self.device} is required")
-        return t.data_ptr(), (t.stride(0) if n > 1 else t.shape[1]), t.shape[1]
+        if t.dtype is self._i32 and t.is_cuda and t.get_device() == self._index and t.dim() == 2:
+            rows, cols = t.shape
+            if rows == n:
+                if t.is_contiguous():
+                    return t.data_ptr(), cols, cols
+                down, along = t.stride()
+                if (cols <= 1 or along == 1) and (n <= 1 or down >= cols):
+                    return t.data_ptr(), (down if n > 1 else cols), cols
+        _refuse(f"table: an int32 tensor [{n}][pages of a request] on {self.device} is required")
 
     def _rows(self, name, t, heads):
         """(address, elements between tokens) of [tokens][heads][hd] with dense rows."""
-        if t.dtype not in self._kinds or t.device != self.device:
+        if t.dtype not in self._kinds or not t.is_cuda or t.get_device() != self._index:
             _refuse(f"{name}: a float32, float16 or bfloat16 tensor on {self.device} is required")
-        if t.dim() != 3 or (heads is not None and t.shape[1] != heads) or t.shape[2] != self.hd:
-            _refuse(f"{name}: shape {tuple(t.shape)}, expected [tokens][{heads or 'heads'}][{self.hd}]")
+        shape, hd = t.shape, self.hd
+        if len(shape) != 3 or (heads is not None and shape[1] != heads) or shape[2] != hd:
+            _refuse(f"{name}: shape {tuple(shape)}, expected [tokens][{heads or 'heads'}][{hd}]")
+        row = shape[1] * hd
+        if t.is_contiguous():
+            return t.data_ptr(), row
         s0, s1, s2 = t.stride()
-        row = t.shape[1] * self.hd
-        if s2 != 1 or (t.shape[1] > 1 and s1 != self.hd) or (t.shape[0] > 1 and s0 < row):
+        if s2 != 1 or (shape[1] > 1 and s1 != hd) or (shape[0] > 1 and s0 < row):
             _refuse(f"{name}: heads and dimensions must be dense within a token")
-        return t.data_ptr(), (s0 if t.shape[0] > 1 else row)
+        return t.data_ptr(), (s0 if shape[0] > 1 else row)
 
     def _pages(self, pages):
         return self._array("pages", pages, self._torch.int32), pages.numel()
@@ -100,29 +123,23 @@ class KVCache:
         starts [n + 1], lens [n] (may be `cached`) and slots of the new tokens
         (tq_kv_plan_dev). free_left: where the remaining count goes (free_count
         itself when None)."""
-        torch = self._torch
-        n = cached.numel()
-        i32 = torch.int32
+        n, i32, array = cached.numel(), self._i32, self._array
         tp, ts, tc = self._table(table, n)
-        left = free_count if free_left is None else free_left
-        a = _lib.KvPlanArgs(n, ts, tc, free_pages.numel(), slots.numel(), self._array("cached", cached, i32),
-                            self._array("added", added, i32, n), tp, self._array("free_pages", free_pages, i32),
-                            self._array("free_count", free_count, i32, 1), self._array("starts", starts, i32, n + 1),
-                            self._array("lens", lens, i32, n), self._array("slots", slots, torch.int64),
-                            self._array("free_left", left, i32, 1))
-        _lib.check(self._L.tq_kv_plan_dev(self._h, ctypes.byref(a), self._stream(stream)))
+        a = _PLAN(n, ts, tc, free_pages.numel(), slots.numel(), array("cached", cached, i32), array("added", added, i32, n),
+                  tp, array("free_pages", free_pages, i32), array("free_count", free_count, i32, 1),
+                  array("starts", starts, i32, n + 1), array("lens", lens, i32, n), array("slots", slots, self._i64),
+                  array("free_left", free_count if free_left is None else free_left, i32, 1))
+        _lib.check(self._L.tq_kv_plan_dev(self._h, a, self._stream(stream)))
 
     def release(self, done, lens, table, free_pages, free_count, free_left=None, stream=None) -> None:
         """Puts the pages of the requests with done != 0 (int32) back on the
         free list and sets their lens to 0 (tq_kv_release_dev)."""
-        n = lens.numel()
-        i32 = self._torch.int32
+        n, i32, array = lens.numel(), self._i32, self._array
         tp, ts, tc = self._table(table, n)
-        left = free_count if free_left is None else free_left
-        a = _lib.KvReleaseArgs(n, ts, tc, free_pages.numel(), self._array("done", done, i32, n),
-                               self._array("lens", lens, i32), tp, self._array("free_pages", free_pages, i32),
-                               self._array("free_count", free_count, i32, 1), self._array("free_left", left, i32, 1))
-        _lib.check(self._L.tq_kv_release_dev(self._h, ctypes.byref(a), self._stream(stream)))
+        a = _RELEASE(n, ts, tc, free_pages.numel(), array("done", done, i32, n), array("lens", lens, i32), tp,
+                     array("free_pages", free_pages, i32), array("free_count", free_count, i32, 1),
+                     array("free_left", free_count if free_left is None else free_left, i32, 1))
+        _lib.check(self._L.tq_kv_release_dev(self._h, a, self._stream(stream)))
 
     # ---- store and attention ----
     def store(self, layer: int, k, v, slots, stream=None) -> None:
@@ -160,12 +177,11 @@ class KVCache:
                 workspace = self._spaces.get(st)
                 if workspace is None:
                     workspace = self._spaces[st] = self.workspace(stream)
-        a = _lib.KvAttentionArgs(qp, op, self._kinds[q.dtype], q.shape[1], q.shape[0], n, qs, os,
-                                 self._array("starts", starts, torch.int32, n + 1),
-                                 self._array("lens", lens, torch.int32), tp, ts, tc,
-                                 self.hd ** -0.5 if scale is None else scale,
-                                 self._array("workspace", workspace, torch.uint8), workspace.numel())
-        _lib.check(self._L.tq_kv_attention_dev(self._h, layer, ctypes.byref(a), st))
+        a = _ATTENTION(qp, op, self._kinds[q.dtype], q.shape[1], q.shape[0], n, qs, os,
+                       self._array("starts", starts, self._i32, n + 1), self._array("lens", lens, self._i32), tp, ts, tc,
+                       self.hd ** -0.5 if scale is None else scale,
+                       self._array("workspace", workspace, torch.uint8), workspace.numel())
+        _lib.check(self._L.tq_kv_attention_dev(self._h, layer, a, st))
         return out
 
     def workspace(self, stream=None):

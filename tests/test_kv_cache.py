@@ -82,3 +82,14 @@ def test_restated_attention_of_one_position_is_its_value():
     ref.store(x, x, np.array([0]))
     out, mag, _, _ = ref.attention(x, [0, 1], [1], np.zeros((1, 1), int), 0.25)
     assert np.array_equal(out[0, 0], ref.values(1, np.array([0]))[0, 0, 0]) and np.array_equal(mag, np.abs(out))
+
+
+def test_packed_arguments_are_the_structs_of_the_header():
+    """kvcache.py packs its arguments; the ctypes structs state the header's layout."""
+    from tensai_b200 import kvcache as K
+    a = K._PLAN(1, 2, 3, 4, 5, *range(6, 15))
+    s = _lib.KvPlanArgs(1, 2, 3, 4, 5, *range(6, 15))
+    assert a == bytes(s)
+    assert K._RELEASE(*range(1, 11)) == bytes(_lib.KvReleaseArgs(*range(1, 11)))
+    v = (1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 11, 12, 13, 0.5, 15, 16)
+    assert K._ATTENTION(*v) == bytes(_lib.KvAttentionArgs(*v))
