@@ -30,6 +30,7 @@
 // CTA, the CTA's in the CTA that arrives last, in a fixed order: results do not
 // depend on timing.
 #include <climits>
+#include <type_traits>
 
 #include "tq_kv_attn.cuh"
 
@@ -72,9 +73,14 @@ __global__ void __launch_bounds__(32 * warps_of(HDP), 1) kv_attn_kernel(const __
     __shared__ long long e_seg[2 * NW], e_end[2 * NW]; // unfinished segments of the warps: first and last tile + 1
     __shared__ int e_row[2 * NW][3];                   // their sequence, KV head, row tile
     __shared__ const float *e_at[2 * NW];              // and where their sums are
-    __shared__ int s_list[2 * NW], s_count;
+    // jobs: the first of their places in s_list, how many partials (of this CTA; wide: of all), the
+    // rows before them (wide: their rows), the first CTA of a segment that others share
+    struct Job {
+        int at, k, row0, from;
+    };
+    __shared__ Job s_job[2 * NW], s_wide[2];
+    __shared__ int s_list[2 * NW], s_jobs, s_rows, s_wides, s_last[2];
     __shared__ volatile int s_late[NW];
-    __shared__ int s_shared[2][3], s_last[2]; // segments that other CTAs share: their place here, first and last CTA
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const int n = p.a.n, n_kv = p.c.n_kv, group = p.group;
 
@@ -551,64 +557,74 @@ __global__ void __launch_bounds__(32 * warps_of(HDP), 1) kv_attn_kernel(const __
     __syncthreads();
 
     // ---- join the warps' unfinished segments, then the CTAs' ------------------------------
-    // the places in use, in order: a segment's are neighbours
+    // The places in use, in order: a segment's are neighbours, and make a job. Its
+    // rows are joined a warp each, so that many short segments go side by side.
     if (warp == 0) {
         const bool used = lane < 2 * NW && e_seg[lane] >= 0;
-        const unsigned all = __ballot_sync(0xffffffffu, used);
-        if (used) s_list[__popc(all & ((1u << lane) - 1))] = lane;
-        if (lane == 0) s_count = __popc(all);
+        const unsigned all = __ballot_sync(0xffffffffu, used), below = (1u << lane) - 1;
+        if (used) s_list[__popc(all & below)] = lane;
+        __syncwarp();
+        const int count = __popc(all), e = lane < count ? s_list[lane] : 0;
+        const long long seg = lane < count ? e_seg[e] : -1, before = __shfl_up_sync(0xffffffffu, seg, 1);
+        const bool first = lane < count && (lane == 0 || seg != before);
+        const unsigned firsts = __ballot_sync(0xffffffffu, first);
+        int rows = 0;
+        if (first) rows = min(R, seq_of(e_row[e][0]).nq * group - e_row[e][2] * R);
+        int upto = rows;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += v;
+        }
+        const bool wide = first && (seg < c0 || e_end[e] > c1); // other CTAs share it: this CTA's first or last
+        const unsigned wides = __ballot_sync(0xffffffffu, wide);
+        if (first) {
+            Job &b = s_job[__popc(firsts & below)];
+            b.at = lane;
+            b.k = (firsts & ~below & ~(1u << lane) ? __ffs(firsts & ~below & ~(1u << lane)) - 1 : count) - lane;
+            b.row0 = upto - rows;
+            b.from = wide ? split.owner(seg) : -1;
+            if (wide) {
+                Job &w = s_wide[__popc(wides & below)];
+                w.at = lane;
+                w.from = b.from;
+                w.k = split.owner(e_end[e] - 1) - b.from + 1;
+                w.row0 = rows;
+            }
+        }
+        if (lane == 31) s_rows = upto;
+        if (lane == 0) s_jobs = __popc(firsts), s_wides = __popc(wides);
     }
     __syncthreads();
-    // Job after job, one piece of code: the segments of this CTA; then, once it has
-    // arrived for those that others share (two at most, the first and the last),
-    // those that it was the last to arrive for.
-    const float **ptr = reinterpret_cast<const float **>(sm + sizeof(float) * partial_floats(HDP)); // over warp 0's ring
-    unsigned *counters = static_cast<unsigned *>(p.a.workspace);
-    int a = 0, shared = 0, done = -1;
-    for (;;) {
-        int k, i, head, rt;
-        float *to = nullptr; // where the sum goes: a partial, or the output
-        if (a < s_count) {
-            const int e = s_list[a];
-            const long long seg = e_seg[e], end = e_end[e];
-            for (k = 1; a + k < s_count && e_seg[s_list[a + k]] == seg; k++) {
-            }
-            i = e_row[e][0], head = e_row[e][1], rt = e_row[e][2];
-            if (tid < k) ptr[tid] = e_at[s_list[a + tid]];
-            if (seg < c0 || end > c1) {
-                const int first = split.owner(seg);
-                to = partial_at(blockIdx.x, (int)blockIdx.x == first ? 1 : 0);
-                if (tid == 0) s_shared[shared][0] = e, s_shared[shared][1] = first, s_shared[shared][2] = split.owner(end - 1);
-                shared++;
-            }
-            a += k;
-        } else {
-            if (shared == 0) break;
-            if (done < 0) {
-                __syncthreads(); // the partials are written
-                if (tid < shared)
-                    s_last[tid] = tq_arrive_last(counters + s_shared[tid][1], s_shared[tid][2] - s_shared[tid][1] + 1);
-                __syncthreads();
-                done = 0;
-            }
-            while (done < shared && !s_last[done]) done++;
-            if (done == shared) break;
-            const int e = s_shared[done][0], first = s_shared[done][1];
-            k = s_shared[done][2] - first + 1;
-            i = e_row[e][0], head = e_row[e][1], rt = e_row[e][2];
-            done++;
-        }
-        __syncthreads();
-        // the sum of the k partials; a thread: 4 dimensions of a row at a time, kAhead partials on their way
-        constexpr int kAhead = 8;
-        const Seq s = seq_of(i);
-        const int rows = min(R, s.nq * group - rt * R);
-        for (int e = tid; e < rows * (HDP / 4); e += NT) {
-            const int r = e / (HDP / 4), d = (e - r * (HDP / 4)) * 4;
+    if (s_jobs == 0) return;
+    // The sum of row r over k partials, partial(j), by a warp: to a partial or, without one, to the output.
+    // mine: partials of this CTA, in shared memory or the workspace.
+    auto join_row = [&](auto partial, auto mine, int k, int r, int e, float *to) {
+        constexpr int kAhead = 8; // partials on their way at once
+        const int i = e_row[e][0], head = e_row[e][1], row = e_row[e][2] * R + r;
+        const int tok = row / group, hq = head * group + row - tok * group;
+        T *o = static_cast<T *>(p.a.out) + (size_t)(seq_of(i).start + tok) * p.a.out_stride + (size_t)hq * p.c.hd;
+        for (int d = 4 * lane; d < HDP; d += 128) {
             float M = -INFINITY, L = 0.f;
             float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
-            auto add = [&](const float (&m)[kAhead], const float (&l)[kAhead], const float4 (&y)[kAhead]) {
-                float top = M;
+#pragma unroll 1
+            for (int j0 = 0; j0 < k; j0 += kAhead) {
+                float m[kAhead], l[kAhead], top = M;
+                float4 y[kAhead];
+#pragma unroll
+                for (int u = 0; u < kAhead; u++) { // the last again, at no weight, beyond the end
+                    const float *f = partial(min(j0 + u, k - 1));
+                    if constexpr (mine.value) {
+                        m[u] = f[16 * PP + r];
+                        l[u] = f[16 * PP + 16 + r];
+                        y[u] = *reinterpret_cast<const float4 *>(f + r * PP + d);
+                    } else {
+                        m[u] = __ldcg(f + 16 * PP + r);
+                        l[u] = __ldcg(f + 16 * PP + 16 + r);
+                        y[u] = __ldcg(reinterpret_cast<const float4 *>(f + r * PP + d));
+                    }
+                    if (j0 + u >= k) m[u] = -INFINITY;
+                }
 #pragma unroll
                 for (int u = 0; u < kAhead; u++) top = fmaxf(top, m[u]);
                 const float base = top == -INFINITY ? 0.f : top, old = exp2f(M - base);
@@ -623,49 +639,32 @@ __global__ void __launch_bounds__(32 * warps_of(HDP), 1) kv_attn_kernel(const __
                     A.z += w * y[u].z;
                     A.w += w * y[u].w;
                 }
-            };
-            float m[kAhead], l[kAhead];
-            float4 y[kAhead];
-            if (done < 0) { // this CTA's: in shared memory, but for some in the workspace
-#pragma unroll 1
-                for (int j0 = 0; j0 < k; j0 += kAhead) {
-#pragma unroll
-                    for (int u = 0; u < kAhead; u++) { // the last again, at no weight, beyond the end
-                        const float *f = ptr[min(j0 + u, k - 1)];
-                        m[u] = f[16 * PP + r];
-                        l[u] = f[16 * PP + 16 + r];
-                        y[u] = *reinterpret_cast<const float4 *>(f + r * PP + d);
-                        if (j0 + u >= k) m[u] = -INFINITY;
-                    }
-                    add(m, l, y);
-                }
-            } else {
-#pragma unroll 1
-                for (int j0 = 0; j0 < k; j0 += kAhead) {
-#pragma unroll
-                    for (int u = 0; u < kAhead; u++) {
-                        const int j = min(j0 + u, k - 1);
-                        const float *f = partial_at(s_shared[done - 1][1] + j, j == 0 ? 1 : 0);
-                        m[u] = __ldcg(f + 16 * PP + r);
-                        l[u] = __ldcg(f + 16 * PP + 16 + r);
-                        y[u] = __ldcg(reinterpret_cast<const float4 *>(f + r * PP + d));
-                        if (j0 + u >= k) m[u] = -INFINITY;
-                    }
-                    add(m, l, y);
-                }
             }
             if (to) {
                 *reinterpret_cast<float4 *>(to + r * PP + d) = A;
                 if (d == 0) to[16 * PP + r] = M, to[16 * PP + 16 + r] = L;
             } else if (d < p.c.hd) {
-                const int row = rt * R + r, tok = row / group, hq = head * group + row - tok * group;
-                T *o = static_cast<T *>(p.a.out) + (size_t)(s.start + tok) * p.a.out_stride + (size_t)hq * p.c.hd + d;
                 const float inv = L == 0.f ? 0.f : 1.f / L;
-                Elem<T>::put2(o, A.x * inv, A.y * inv, p.vec, true);
-                Elem<T>::put2(o + 2, A.z * inv, A.w * inv, p.vec, true);
+                Elem<T>::put2(o + d, A.x * inv, A.y * inv, p.vec, true);
+                Elem<T>::put2(o + d + 2, A.z * inv, A.w * inv, p.vec, true);
             }
         }
-        __syncthreads(); // the pointers are read
+    };
+    for (int item = warp; item < s_rows; item += NW) {
+        const Job b = s_job[__popc(__ballot_sync(0xffffffffu, lane < s_jobs && s_job[lane < s_jobs ? lane : 0].row0 <= item)) - 1];
+        float *to = b.from < 0 ? nullptr : partial_at(blockIdx.x, (int)blockIdx.x == b.from ? 1 : 0);
+        join_row([&](int j) { return e_at[s_list[b.at + j]]; }, std::true_type(), b.k, item - b.row0, s_list[b.at], to);
+    }
+    if (s_wides == 0) return;
+    __syncthreads(); // the partials are written
+    unsigned *counters = static_cast<unsigned *>(p.a.workspace);
+    if (tid < s_wides) s_last[tid] = tq_arrive_last(counters + s_wide[tid].from, s_wide[tid].k);
+    __syncthreads();
+    const int rows0 = s_last[0] ? s_wide[0].row0 : 0, rows1 = s_wides > 1 && s_last[1] ? s_wide[1].row0 : 0;
+    for (int item = warp; item < rows0 + rows1; item += NW) {
+        const Job b = s_wide[item < rows0 ? 0 : 1];
+        join_row([&](int j) { return (const float *)partial_at(b.from + j, j == 0 ? 1 : 0); }, std::false_type(), b.k,
+                 item < rows0 ? item : item - rows0, s_list[b.at], nullptr);
     }
 }
 
