@@ -6,7 +6,7 @@
 // cut into blocks of 256, two tiles A and B of 128 rows, positions into tiles of
 // 128. For each position tile and row tile:
 //   S = Q K^T    tcgen05.mma kind::f16, operands in shared memory, S in TMEM;
-//   softmax      one thread a row: S from TMEM, P back over S as float16;
+//   softmax      two threads a row: S from TMEM, P back over S as float16;
 //   O += P V     tcgen05.mma with P from TMEM, O in TMEM.
 // While the softmax of one row tile runs, the tensor cores work for the other.
 // Codes become float16 once per CTA and position tile (exact), in four warps
@@ -41,7 +41,8 @@ constexpr int kRows = 128;      // rows of a tile
 constexpr int kBlockRows = 256; // rows of a block: tiles A and B
 constexpr int kPos = 128;       // positions of a tile
 constexpr int kBlocks = kPos / TQ_KV_BLOCK;
-constexpr int kSoftWarps = 8, kConvWarps = 4;
+constexpr int kSoftWarps = 16, kConvWarps = 4;
+constexpr int kTileThreads = 2 * kRows; // softmax threads of a row tile: two a row, half the columns each
 constexpr int kConvThreads = 32 * kConvWarps;
 constexpr int kMmaWarp = kSoftWarps + kConvWarps; // one thread of it issues; the next warp loads
 constexpr int kThreads = 32 * (kMmaWarp + 2);
@@ -56,7 +57,7 @@ constexpr int kJoinThreads = 256, kJoinRows = 32;
 constexpr int stages_of(int hdp, int pieces) { return hdp == 128 && pieces == 2 ? 1 : 2; }
 constexpr size_t operand_bytes(int hdp) { return (size_t)kPos * hdp * 2; } // a K or V tile, or a piece of a Q tile
 constexpr size_t smem_bytes(int hdp, int pieces) {
-    return 1024 + operand_bytes(hdp) * (2 * pieces + 2 * stages_of(hdp, pieces) + 1); // the staged codes are one more
+    return 3072 + operand_bytes(hdp) * (2 * pieces + 2 * stages_of(hdp, pieces) + 1); // struct Shared; the staged codes are one more
 }
 constexpr size_t partial_floats(int hdp) { return (size_t)kBlockRows * (hdp + 2); }
 
@@ -104,9 +105,9 @@ __device__ __forceinline__ Seq prompt_seq(const Params &p, int i) {
 }
 
 // sums[e] = units of the sequences before entry e, for all threads of a block; the total.
-template <int NT> __device__ __forceinline__ long long list_sums(const Params &p, long long *sums) {
+// scan: a word for each warp.
+template <int NT> __device__ __forceinline__ long long list_sums(const Params &p, long long *sums, long long *scan) {
     constexpr int NW = NT / 32, PER = (kKvSums + NT - 1) / NT;
-    __shared__ long long scan[NW];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int n = p.a.n, entries = (n + (1 << p.shift_sums) - 1) >> p.shift_sums;
     for (int e = tid; e < entries; e += NT) sums[e] = 0;
@@ -241,22 +242,16 @@ __device__ __forceinline__ int tiles_of(const Where &w, int t, int group) {
 
 // ---- tensor memory and MMA -------------------------------------------------------------
 
-__device__ __forceinline__ void tmem_ld32(uint32_t a, uint32_t (&v)[32]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
-        "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
-          "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]),
-          "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]),
-          "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
-        : "r"(a)
-        : "memory");
-}
 __device__ __forceinline__ void tmem_st16(uint32_t a, const uint32_t (&v)[16]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(
                      a),
                  "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]),
                  "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t a, const uint32_t (&v)[16]) { // the first 8
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(a), "r"(v[0]), "r"(v[1]),
+                 "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
                  : "memory");
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -305,7 +300,7 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return y;
 }
 
-struct Shared { // static shared memory
+struct Shared { // behind the operands
     uint64_t seg_full[kSegs], seg_empty[kSegs];
     uint64_t code_full[2], code_empty[2]; // staged codes: keys, values
     uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
@@ -313,27 +308,28 @@ struct Shared { // static shared memory
     Seg seg[kSegs];
     float f[kConsts][kBlocks], lv[kConsts][kBlocks], rv[kConsts][kBlocks];
     unsigned poison[kConsts]; // blocks with a scale that is not a number
-    float back[2][kRows]; // what a row of Q was divided by
+    // between the two threads of a row: w, at the end L; before the first w, what its Q was divided by
+    float swap[2][2][kRows];
     unsigned live[2]; // blocks of the staged keys, values that are there (values: and not all zero)
     uint32_t tmem;
     volatile int late;
 };
+static_assert(sizeof(Shared) <= 3072, "the room behind the operands");
 
 template <int HDP, int PIECES, typename T>
 __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const __grid_constant__ Params p) {
     constexpr int ST = stages_of(HDP, PIECES);
     constexpr uint32_t OP = (uint32_t)operand_bytes(HDP), CODES = (uint32_t)kPos * HDP;
-    extern __shared__ unsigned char raw[];
-    __shared__ __align__(16) Shared sh;
-    unsigned char *base = reinterpret_cast<unsigned char *>(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
-    unsigned char *Qs = base;                 // [2 tiles][PIECES][OP]
+    extern __shared__ __align__(1024) unsigned char raw[];
+    unsigned char *Qs = raw;                  // [2 tiles][PIECES][OP]
     unsigned char *Ks = Qs + 2 * PIECES * OP; // [ST][OP]
     unsigned char *Vs = Ks + ST * OP;         // [ST][OP]
     unsigned char *Cs = Vs + ST * OP;         // [keys, values][CODES]: as the cache holds them
+    Shared &sh = *reinterpret_cast<Shared *>(Cs + 2 * CODES);
     long long *sums = reinterpret_cast<long long *>(Cs); // before the first codes
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int group = p.group;
-    const long long total = list_sums<kThreads>(p, sums);
+    const long long total = list_sums<kThreads>(p, sums, sums + kKvSums + 1);
     const int G = (int)min((long long)gridDim.x, (total + kMinUnits - 1) / kMinUnits);
     if ((int)blockIdx.x >= G) return; // none: G = 0
 
@@ -349,8 +345,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const __grid_con
             tqp::mbar_init(&sh.v_full[s], kConvThreads);
             tqp::mbar_init(&sh.k_empty[s], 1);
             tqp::mbar_init(&sh.v_empty[s], 1);
-            tqp::mbar_init(&sh.q_ready[s], kRows);
-            tqp::mbar_init(&sh.p_ready[s], kRows);
+            tqp::mbar_init(&sh.q_ready[s], kTileThreads);
+            tqp::mbar_init(&sh.p_ready[s], kTileThreads);
             tqp::mbar_init(&sh.s_full[s], 1);
             tqp::mbar_init(&sh.o_full[s], 1);
         }
@@ -376,53 +372,59 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const __grid_con
     };
 
     if (warp < kSoftWarps) {
-        // ================= softmax: thread = row of tile t =================
-        const int t = warp >> 2, row = (warp & 3) * 32 + lane;
+        // ================= softmax: thread = half a row of tile t =================
+        const int t = warp >> 3, half = warp >> 2 & 1, row = (warp & 3) * 32 + lane;
+        constexpr int OC = HDP / 2; // columns of O that a thread has
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-        const uint32_t s_at = s_col(t) + lanes, o_at = o_col(t) + lanes;
+        const uint32_t s_at = s_col(t) + lanes + half * (kPos / 2), o_at = o_col(t) + lanes + half * OC;
+        float *put = &sh.swap[t][half][row], *get = &sh.swap[t][1 - half][row];
+        auto together = [&]() { tqp::named_sync(1 + t, kTileThreads); };
         unsigned tick = 0, s_phase = 0, o_phase = 0; // position tiles of the CTA so far; barrier phases
         for (unsigned n = 0;; n++) {
             const Seg &g = next_seg(n);
             const int cnt = g.cnt, mine = g.mine[t], tile0 = g.tile, part_at = g.part;
             if (cnt == 0) break;
-            const int row0 = g.row0, head = g.head, start = g.start, rows = g.nq * group;
-            const int r = row0 + t * kRows + row;
+            const int row0 = g.row0 + t * kRows, head = g.head, start = g.start, rows = g.nq * group;
             const int len = g.len, fresh = g.nq;
             __syncwarp();
             if (lane == 0) tqp::mbar_arrive(&sh.seg_empty[n % kSegs]);
-            // the row's place among the queries and the outputs, -1 for a row that is not there
-            const int tok = r / group, hq = head * group + r - tok * group;
-            const long long q_at = r < rows ? (long long)(start + tok) * p.a.q_stride + (long long)hq * p.c.hd : -1;
-            const long long o_at_row = r < rows ? (long long)(start + tok) * p.a.out_stride + (long long)hq * p.c.hd : -1;
-            const int lim = r < rows ? min(len, max(0, len - fresh + tok + 1)) : len;
+            // a row's place among the queries or the outputs, -1 for a row that is not there
+            auto place = [&](int r, long long stride) {
+                const int tok = r / group, hq = head * group + r - tok * group;
+                return r < rows ? (long long)(start + tok) * stride + (long long)hq * p.c.hd : -1;
+            };
+            const int r = row0 + row;
+            const int lim = r < rows ? min(len, max(0, len - fresh + r / group + 1)) : len;
             float M = -INFINITY, L = 0.f;
             if (mine > 0) {
-                // ---- Q, as float16 pieces: the warp's 32 rows, each by as many lanes as it has 16-byte words.
+                // ---- Q, as float16 pieces: 16 rows a warp, each by as many lanes as it has 16-byte words.
                 // The words come into the row's own memory (128 bytes for each 64 dimensions and piece)
                 // and are replaced there by the pieces.
                 constexpr int E = 16 / sizeof(T), LANES = HDP / E, ROWS = 32 / LANES;
                 unsigned char *qs = Qs + t * PIECES * OP;
-                const int word = lane % LANES, d = word * E, sub = lane / LANES;
+                const int word = lane % LANES, d = word * E, sub = lane / LANES, first = (warp & 7) * 16;
+                const long long q_at = place(row0 + first + (lane & 15), p.a.q_stride);
                 auto raw_at = [&](int qrow) {
                     return reinterpret_cast<uint4 *>(qs + (word >> 3) * (kRows * 128) + chunk_at(qrow, word & 7));
                 };
                 constexpr int BATCH = 4; // rows a lane works on at once
+                together(); // the last segment's outputs have left this memory
                 if (p.vec) {
 #pragma unroll 4
-                    for (int i = 0; i < 32; i += ROWS) {
+                    for (int i = 0; i < 16; i += ROWS) {
                         const long long at = __shfl_sync(0xffffffffu, q_at, i + sub);
                         const bool there = at >= 0 && d < p.c.hd;
                         asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
-                                         tqp::smem_u32(raw_at((warp & 3) * 32 + i + sub))),
+                                         tqp::smem_u32(raw_at(first + i + sub))),
                                      "l"(static_cast<const T *>(p.a.q) + (there ? at + d : 0)), "r"(there ? 16 : 0)
                                      : "memory");
                     }
                 } else {
 #pragma unroll 1
-                    for (int i = 0; i < 32; i += ROWS) {
+                    for (int i = 0; i < 16; i += ROWS) {
                         const long long at = __shfl_sync(0xffffffffu, q_at, i + sub);
                         const bool there = at >= 0 && d < p.c.hd;
-                        T *to = reinterpret_cast<T *>(raw_at((warp & 3) * 32 + i + sub));
+                        T *to = reinterpret_cast<T *>(raw_at(first + i + sub));
 #pragma unroll 1
                         for (int e = 0; e < E; e++) to[e] = there ? static_cast<const T *>(p.a.q)[at + d + e] : T(0.f);
                     }
@@ -430,11 +432,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const __grid_con
                 asm volatile("cp.async.wait_all;" ::: "memory");
                 __syncwarp();
 #pragma unroll 1
-                for (int i = 0; i < 32; i += ROWS * BATCH) {
+                for (int i = 0; i < 16; i += ROWS * BATCH) {
                     uint4 w[BATCH];
                     float big[BATCH];
 #pragma unroll
-                    for (int u = 0; u < BATCH; u++) w[u] = *raw_at((warp & 3) * 32 + i + u * ROWS + sub);
+                    for (int u = 0; u < BATCH; u++) w[u] = *raw_at(first + i + u * ROWS + sub);
 #pragma unroll
                     for (int u = 0; u < BATCH; u++) {
                         big[u] = 0.f;
@@ -448,10 +450,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const __grid_con
                         for (int u = 0; u < BATCH; u++) big[u] = fmaxf(big[u], __shfl_xor_sync(0xffffffffu, big[u], o));
 #pragma unroll
                     for (int u = 0; u < BATCH; u++) {
-                        const int qrow = (warp & 3) * 32 + i + u * ROWS + sub;
+                        const int qrow = first + i + u * ROWS + sub;
                         float was, unit = row_scale(big[u], &was);
                         if (p.scale2 < 0.f) unit = -unit; // the block factors stay positive
-                        if (word == 0) sh.back[t][qrow] = was;
+                        if (word < 2) sh.swap[t][word][qrow] = was;
                         unsigned hi[E / 2], lo[E / 2];
 #pragma unroll
                         for (int e = 0; e < E / 2; e++) {
@@ -471,39 +473,37 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const __grid_con
                     }
                 }
                 static_assert((sizeof(T) == 4) == (PIECES == 2), "a row's pieces take the room of its elements");
-                __syncwarp();
-                const float back = sh.back[t][row];
                 tqp::fence_proxy_async();
+                together();
+                const float back = *put;
                 tqp::tc_fence_before(); // the last segment's reads of S and O
                 tqp::mbar_arrive(&sh.q_ready[t]);
 
                 for (int j = 0; j < mine; j++) {
-                    const int cs = (tick + j) % kConsts;
-                    const int seen = lim - (tile0 + j) * kPos; // columns below it are visible
-                    const bool whole = __all_sync(0xffffffffu, seen >= kPos);
+                    const int cs = (tick + j) % kConsts, b0 = half * (kBlocks / 2);
+                    const int seen = lim - (tile0 + j) * kPos - half * (kPos / 2); // this half's columns below it are visible
+                    const bool whole = __all_sync(0xffffffffu, seen >= kPos / 2);
                     wait_slot(&sh.s_full[t], s_phase & 1, &sh.late, p.c.status);
                     s_phase++;
                     tqp::tc_fence_after();
-                    // S comes through 32 registers at a time, the next 32 on their way; the
-                    // loops are kept short: straight code of a whole row runs at the rate
-                    // at which instructions arrive.
+                    // S comes a block of 16 columns at a time, the next on its way
                     auto over = [&](auto &&use) {
-                        uint32_t v0[32], v1[32];
-                        tmem_ld32(s_at, v0);
+                        uint32_t v0[16], v1[16];
+                        tqp::tmem_ld16(s_at, v0);
                         tqp::tmem_wait_ld();
 #pragma unroll 1
-                        for (int c = 0; c < 4; c += 2) {
-                            tmem_ld32(s_at + 32 * (c + 1), v1);
-                            use(c, v0);
+                        for (int b = 0; b < kBlocks / 2; b += 2) {
+                            tqp::tmem_ld16(s_at + 16 * (b + 1), v1);
+                            use(b, v0);
                             tqp::tmem_wait_ld();
-                            if (c == 0) tmem_ld32(s_at + 64, v0);
-                            use(c + 1, v1);
+                            if (b + 2 < kBlocks / 2) tqp::tmem_ld16(s_at + 16 * (b + 2), v0);
+                            use(b + 1, v1);
                             tqp::tmem_wait_ld();
                         }
                     };
                     if (!whole) { // what a row does not see
 #pragma unroll 1
-                        for (int c = 0; c < kPos; c += 16) {
+                        for (int c = 0; c < kPos / 2; c += 16) {
                             uint32_t v[16];
                             tqp::tmem_ld16(s_at + c, v);
                             tqp::tmem_wait_ld();
@@ -516,17 +516,16 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const __grid_con
                     }
                     // ---- M ----
                     float top = -INFINITY;
-                    over([&](int c, const uint32_t (&v)[32]) {
+                    over([&](int b, const uint32_t (&v)[16]) {
+                        float mx = __uint_as_float(v[0]);
 #pragma unroll
-                        for (int b = 0; b < 2; b++) {
-                            float mx = __uint_as_float(v[16 * b]);
-#pragma unroll
-                            for (int u = 1; u < 15; u += 2)
-                                mx = max3(mx, __uint_as_float(v[16 * b + u]), __uint_as_float(v[16 * b + u + 1]));
-                            mx = fmaxf(mx, __uint_as_float(v[16 * b + 15]));
-                            top = fmaxf(top, fmaf(mx, sh.f[cs][2 * c + b] * back, sh.lv[cs][2 * c + b]));
-                        }
+                        for (int u = 1; u < 15; u += 2) mx = max3(mx, __uint_as_float(v[u]), __uint_as_float(v[u + 1]));
+                        mx = fmaxf(mx, __uint_as_float(v[15]));
+                        top = fmaxf(top, fmaf(mx, sh.f[cs][b0 + b] * back, sh.lv[cs][b0 + b]));
                     });
+                    *put = top;
+                    together();
+                    top = fmaxf(top, *get);
                     if (top > M + kSlack) {
                         const float alpha = ex2(M - top);
                         M = top;
@@ -538,69 +537,68 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const __grid_con
                     if (j > 0 && __any_sync(0xffffffffu, top != 1.f)) {
                         // S of this tile is complete, so O += P V of the last one is (issued before it)
 #pragma unroll 1
-                        for (int c = 0; c < HDP / 16; c++) {
+                        for (int c = 0; c < OC; c += 16) {
                             uint32_t o[16];
-                            tqp::tmem_ld16(o_at + 16 * c, o);
+                            tqp::tmem_ld16(o_at + c, o);
                             tqp::tmem_wait_ld();
 #pragma unroll
                             for (int u = 0; u < 16; u++) o[u] = __float_as_uint(__uint_as_float(o[u]) * top);
-                            tmem_st16(o_at + 16 * c, o);
+                            tmem_st16(o_at + c, o);
                         }
                     }
-                    // ---- P over S: chunk c's 16 (or, in two pieces, 32) columns lie in columns already read ----
+                    // ---- P over S: a block's 8 (or, in two pieces, 16) columns lie in columns already read ----
                     const float use = M == -INFINITY ? 0.f : M - kUnit;
-                    over([&](int c, const uint32_t (&v)[32]) {
-                        uint32_t hi[16], lo[16];
+                    over([&](int b, const uint32_t (&v)[16]) {
+                        uint32_t y[16];
+                        const float fb = sh.f[cs][b0 + b] * back, ob = sh.lv[cs][b0 + b] - use;
+                        float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
-                        for (int b = 0; b < 2; b++) {
-                            const float fb = sh.f[cs][2 * c + b] * back, ob = sh.lv[cs][2 * c + b] - use;
-                            float2 sum = make_float2(0.f, 0.f);
-#pragma unroll
-                            for (int u = 0; u < 16; u += 2) {
-                                const float2 s = make_float2(__uint_as_float(v[16 * b + u]), __uint_as_float(v[16 * b + u + 1]));
-                                const float2 e = __ffma2_rn(s, make_float2(fb, fb), make_float2(ob, ob));
-                                const float2 y = make_float2(ex2(e.x), ex2(e.y));
-                                sum = __fadd2_rn(sum, y);
-                                const unsigned h = pack2(y.x, y.y);
-                                hi[8 * b + u / 2] = h;
-                                if (PIECES == 2) {
-                                    const float2 z = unpack2(h);
-                                    lo[8 * b + u / 2] = pack2(y.x - z.x, y.y - z.y);
-                                }
+                        for (int u = 0; u < 16; u += 2) {
+                            const float2 s = make_float2(__uint_as_float(v[u]), __uint_as_float(v[u + 1]));
+                            const float2 e = __ffma2_rn(s, make_float2(fb, fb), make_float2(ob, ob));
+                            const float2 x = make_float2(ex2(e.x), ex2(e.y));
+                            sum = __fadd2_rn(sum, x);
+                            y[u / 2] = pack2(x.x, x.y);
+                            if (PIECES == 2) {
+                                const float2 z = unpack2(y[u / 2]);
+                                y[8 + u / 2] = pack2(x.x - z.x, x.y - z.y);
                             }
-                            L = fmaf(sum.x + sum.y, sh.rv[cs][2 * c + b], L);
                         }
-                        if (PIECES == 1) {
-                            tmem_st16(s_at + 16 * c, hi);
-                        } else {
-                            tmem_st16(s_at + 32 * c, hi);
-                            tmem_st16(s_at + 32 * c + 16, lo);
-                        }
+                        L = fmaf(sum.x + sum.y, sh.rv[cs][b0 + b], L);
+                        if (PIECES == 1)
+                            tmem_st8(s_at + 8 * b, y);
+                        else
+                            tmem_st16(s_at + 16 * b, y);
                     });
                     // a scale that is not a number spoils the rows that see its block
-                    for (unsigned bad = sh.poison[cs]; bad; bad &= bad - 1)
+                    for (unsigned bad = sh.poison[cs] >> b0 & 15u; bad; bad &= bad - 1)
                         if (seen > (__ffs(bad) - 1) * TQ_KV_BLOCK) L = __int_as_float(0x7fc00000);
                     tmem_wait_st();
                     tqp::tc_fence_before();
                     tqp::mbar_arrive(&sh.p_ready[t]);
                 }
+                together(); // the last w is read
+                *put = L;
+                together();
+                L += *get;
                 wait_slot(&sh.o_full[t], o_phase & 1, &sh.late, p.c.status);
                 o_phase++;
                 tqp::tc_fence_after();
             }
-            // ---- out, or this part of it: some columns at a time through this warp's own rows of Q's memory
-            // (other warps may be loading theirs for the next segment) ----
-            constexpr int RB = PIECES * OP / kRows < 256 ? PIECES * OP / kRows : 256; // bytes of a row there
-            unsigned char *stage = Qs + t * PIECES * OP + (warp & 3) * (32 * 128);
-            auto staged = [&](int sr, int c) { // 16-byte chunk c of row sr of the warp
-                return reinterpret_cast<uint4 *>(stage + (c >> 3) * (kRows * 128) + sr * 128 + (((c & 7) ^ (sr & 7)) << 4));
+            // ---- out, or this part of it: some columns at a time through the rows' memory of Q, the halves apart ----
+            const long long o_at_row = place(r, p.a.out_stride);
+            constexpr int CH = PIECES * HDP / 16; // 16-byte chunks of a row there for a half
+            auto staged = [&](int sr, int c) {    // chunk c of row sr of the warp
+                const int ch = half * CH + c;
+                return reinterpret_cast<uint4 *>(Qs + t * PIECES * OP + (ch >> 3) * (kRows * 128) +
+                                                 chunk_at((warp & 3) * 32 + sr, ch & 7));
             };
-            auto spread = [&](auto one, float factor, auto &&at) { // one: the element type; at(row of the warp): its address
+            auto spread = [&](auto one, float factor, auto &&at) { // one: the element type
                 using X = decltype(one);
-                constexpr int E = 16 / sizeof(X), COLS = RB / (int)sizeof(X) < HDP ? RB / (int)sizeof(X) : HDP;
+                constexpr int E = 16 / sizeof(X), COLS = CH * E < OC ? CH * E : OC;
                 constexpr int LANES = COLS / E, ROWS = 32 / LANES;
 #pragma unroll 1
-                for (int h = 0; h < HDP; h += COLS) {
+                for (int h = 0; h < OC; h += COLS) {
                     __syncwarp();
 #pragma unroll 1
                     for (int c = 0; c < COLS; c += 16) {
@@ -625,15 +623,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const __grid_con
                         long long to[4];
 #pragma unroll
                         for (int u = 0; u < 4; u++) {
-                            const int sr = (i + u * ROWS + lane / LANES) & 31;
+                            const int sr = i + u * ROWS + lane / LANES;
                             x[u] = *staged(sr, c);
                             to[u] = __shfl_sync(0xffffffffu, o_at_row, sr);
                         }
 #pragma unroll
-                        for (int u = 0; u < 4; u++) {
-                            const int sr = i + u * ROWS + lane / LANES;
-                            if (sr < 32) at(sr, h + c * E, x[u], to[u]);
-                        }
+                        for (int u = 0; u < 4; u++) at(i + u * ROWS + lane / LANES, half * OC + h + c * E, x[u], to[u]);
                     }
                 }
                 __syncwarp();
@@ -658,9 +653,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const __grid_con
                     spread(0.f, 1.f, [&](int sr, int d, const uint4 &x, long long) {
                         *reinterpret_cast<uint4 *>(part + (size_t)(t * kRows + (warp & 3) * 32 + sr) * HDP + d) = x;
                     });
-                const int pr = t * kRows + row;
-                part[kBlockRows * HDP + pr] = mine > 0 ? M : __int_as_float(0x7fc00000); // NaN: no part here
-                part[kBlockRows * HDP + kBlockRows + pr] = L;
+                if (half == 0) {
+                    const int pr = t * kRows + row;
+                    part[kBlockRows * HDP + pr] = mine > 0 ? M : __int_as_float(0x7fc00000); // NaN: no part here
+                    part[kBlockRows * HDP + kBlockRows + pr] = L;
+                }
             }
             tick += cnt;
         }
@@ -751,8 +748,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const __grid_con
                 for (int pc = 0; pc < PIECES; pc++)
 #pragma unroll
                     for (int ks = 0; ks < kPos / 16; ks++) {
-                        const uint32_t a =
-                            PIECES == 1 ? s_col(t) + 8 * ks : s_col(t) + 32 * (ks >> 1) + 16 * pc + 8 * (ks & 1);
+                        const uint32_t a = // a half's blocks lie behind one another (two pieces: side by side)
+                            PIECES == 1 ? s_col(t) + (ks >> 2) * (kPos / 2) + 8 * (ks & 3) : s_col(t) + 16 * ks + 8 * pc;
                         mma_ts(o_col(t), a, desc(vb + (ks >> 2) * (HDP * 128) + (ks & 3) * 32), idesc_f16(HDP),
                                !first || pc > 0 || ks > 0);
                     }
@@ -904,8 +901,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const __grid_con
 // and did not end: 32 rows a block.
 template <int HDP, typename T>
 __global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const __grid_constant__ Params p, int grid) {
-    __shared__ long long sums[kKvSums + 1];
-    const long long total = list_sums<kJoinThreads>(p, sums);
+    __shared__ long long sums[kKvSums + 1], scan[kJoinThreads / 32];
+    const long long total = list_sums<kJoinThreads>(p, sums, scan);
     const int G = (int)min((long long)grid, (total + kMinUnits - 1) / kMinUnits);
     const int cta = blockIdx.x;
     if (cta + 1 >= G) return;
