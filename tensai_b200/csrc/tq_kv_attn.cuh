@@ -135,12 +135,16 @@ __device__ __forceinline__ Seq seq_at(const TqKvParams &p, const int *starts, co
 
 // Bounded wait for an mbarrier. What it waits for always arrives; should it not, the status says so and no later wait of the CTA waits.
 __device__ __forceinline__ void wait_long(uint64_t *bar, unsigned parity, volatile int *late, unsigned *status) {
-    const unsigned long long t0 = tqp::global_ns();
-    while (!*late) {
+    unsigned long long t0 = 0;
+    for (unsigned it = 1; !*late; it++) {
         if (tqp::mbar_try_wait_hint(bar, parity, 200000u)) return;
-        if (tqp::global_ns() - t0 > tqp::kWaitNs) {
-            atomicOr(status, TQ_KV_STATUS_TIMEOUT);
-            *late = 1;
+        if (it % 64 == 0) { // reading the clock costs more than most waits last
+            const unsigned long long now = tqp::global_ns();
+            if (t0 == 0) t0 = now;
+            if (now - t0 > tqp::kWaitNs) {
+                atomicOr(status, TQ_KV_STATUS_TIMEOUT);
+                *late = 1;
+            }
         }
     }
 }

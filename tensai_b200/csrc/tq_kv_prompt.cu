@@ -29,6 +29,7 @@
 // Bound by the exponentials (16 a cycle and SM) and the tensor cores alike: 128
 // positions of 128 rows take about 1024 cycles of each at head size 128.
 #include <climits>
+#include <type_traits>
 
 #include "tq_kv_attn.cuh"
 
@@ -728,59 +729,64 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const __grid_con
     } else if (warp == kMmaWarp) {
         // ================= MMA issue: one thread =================
         if (lane == 0) {
-            unsigned tick = 0, q_phase[2] = {0, 0}, p_phase[2] = {0, 0};
-            const uint32_t q0 = tqp::smem_u32(Qs), k0 = tqp::smem_u32(Ks), v0 = tqp::smem_u32(Vs);
-            auto scores = [&](int t, unsigned n) { // S(t) = Q(t) K(n)^T
-                const uint32_t kb = k0 + (n % ST) * OP;
+            unsigned tick = 0, q_phase = 0, p_phase = 0; // phases: a bit for each row tile
+            // descriptors differ in their address field alone: 16-byte units, no carry out of it
+            const uint64_t dq = desc(tqp::smem_u32(Qs)), dk = desc(tqp::smem_u32(Ks)), dv = desc(tqp::smem_u32(Vs));
+            auto scores = [&](auto t, unsigned n) { // S(t) = Q(t) K(n)^T
+                const uint64_t kb = dk + (n % ST) * (OP >> 4);
 #pragma unroll
                 for (int pc = 0; pc < PIECES; pc++)
 #pragma unroll
                     for (int ks = 0; ks < HDP / 16; ks++) {
-                        const uint32_t o = (ks >> 2) * (kRows * 128) + (ks & 3) * 32;
-                        mma_ss(s_col(t), desc(q0 + (t * PIECES + pc) * OP + o), desc(kb + o), idesc_f16(kPos),
-                               pc > 0 || ks > 0);
+                        const uint32_t o = ((ks >> 2) * (kRows * 128) + (ks & 3) * 32) >> 4;
+                        mma_ss(s_col(t), dq + ((t * PIECES + pc) * (OP >> 4) + o), kb + o, idesc_f16(kPos), pc > 0 || ks > 0);
                     }
                 tqp::umma_commit(&sh.s_full[t]);
             };
-            auto products = [&](int t, unsigned n, bool first) { // O(t) += P(t) V(n)
-                const uint32_t vb = v0 + (n % ST) * OP;
+            auto products = [&](auto t, unsigned n, bool first) { // O(t) += P(t) V(n)
+                const uint64_t vb = dv + (n % ST) * (OP >> 4);
 #pragma unroll
                 for (int pc = 0; pc < PIECES; pc++)
 #pragma unroll
                     for (int ks = 0; ks < kPos / 16; ks++) {
                         const uint32_t a = // a half's blocks lie behind one another (two pieces: side by side)
                             PIECES == 1 ? s_col(t) + (ks >> 2) * (kPos / 2) + 8 * (ks & 3) : s_col(t) + 16 * ks + 8 * pc;
-                        mma_ts(o_col(t), a, desc(vb + (ks >> 2) * (HDP * 128) + (ks & 3) * 32), idesc_f16(HDP),
-                               !first || pc > 0 || ks > 0);
+                        mma_ts(o_col(t), a, vb + (((ks >> 2) * (HDP * 128) + (ks & 3) * 32) >> 4), idesc_f16(HDP),
+                               pc > 0 || ks > 0 ? 1u : !first);
                     }
+            };
+            auto wait_tile = [&](uint64_t *bars, auto t, unsigned &phase) {
+                wait_slot(&bars[t], phase >> t & 1, &sh.late, p.c.status);
+                phase ^= 1u << t;
             };
             for (unsigned sn = 0;; sn++) {
                 const Seg &g = next_seg(sn);
-                const int cnt = g.cnt, mine[2] = {g.mine[0], g.mine[1]};
+                const int cnt = g.cnt, mine_a = g.mine[0], mine_b = g.mine[1];
                 tqp::mbar_arrive(&sh.seg_empty[sn % kSegs]);
                 if (cnt == 0) break;
                 for (int j = -1; j < cnt; j++) {
                     const unsigned n = tick + j;
-#pragma unroll 1
-                    for (int t = 0; t < 2; t++) {
-                        // every tile's operands are waited for once, whether a row tile uses them or not
+                    // every tile's operands are waited for once, whether a row tile uses them or not
+                    auto half_step = [&](auto t, int mine) {
                         if (j >= 0 && t == 0) wait_slot(&sh.v_full[n % ST], (n / ST) & 1, &sh.late, p.c.status);
-                        if (j >= 0 && j < mine[t]) {
-                            wait_slot(&sh.p_ready[t], p_phase[t]++ & 1, &sh.late, p.c.status);
+                        if (j >= 0 && j < mine) {
+                            wait_tile(sh.p_ready, t, p_phase);
                             tqp::tc_fence_after();
                             products(t, n, j == 0);
-                            if (j + 1 == mine[t]) tqp::umma_commit(&sh.o_full[t]);
+                            if (j + 1 == mine) tqp::umma_commit(&sh.o_full[t]);
                         }
                         if (j >= 0 && t == 1) tqp::umma_commit(&sh.v_empty[n % ST]);
                         if (j + 1 < cnt && t == 0)
                             wait_slot(&sh.k_full[(n + 1) % ST], ((n + 1) / ST) & 1, &sh.late, p.c.status);
-                        if (j + 1 < mine[t]) {
-                            if (j < 0) wait_slot(&sh.q_ready[t], q_phase[t]++ & 1, &sh.late, p.c.status);
+                        if (j + 1 < mine) {
+                            if (j < 0) wait_tile(sh.q_ready, t, q_phase);
                             tqp::tc_fence_after();
                             scores(t, n + 1);
                         }
                         if (j + 1 < cnt && t == 1) tqp::umma_commit(&sh.k_empty[(n + 1) % ST]);
-                    }
+                    };
+                    half_step(std::integral_constant<int, 0>(), mine_a);
+                    half_step(std::integral_constant<int, 1>(), mine_b);
                 }
                 tick += cnt;
             }
