@@ -342,12 +342,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const __grid_con
         for (int s = 0; s < 2; s++) {
             tqp::mbar_init(&sh.code_full[s], 1);
             tqp::mbar_init(&sh.code_empty[s], kConvWarps);
-            tqp::mbar_init(&sh.k_full[s], kConvThreads);
-            tqp::mbar_init(&sh.v_full[s], kConvThreads);
+            tqp::mbar_init(&sh.k_full[s], kConvWarps);
+            tqp::mbar_init(&sh.v_full[s], kConvWarps);
             tqp::mbar_init(&sh.k_empty[s], 1);
             tqp::mbar_init(&sh.v_empty[s], 1);
-            tqp::mbar_init(&sh.q_ready[s], kTileThreads);
-            tqp::mbar_init(&sh.p_ready[s], kTileThreads);
+            tqp::mbar_init(&sh.q_ready[s], kTileThreads / 32);
+            tqp::mbar_init(&sh.p_ready[s], kTileThreads / 32);
             tqp::mbar_init(&sh.s_full[s], 1);
             tqp::mbar_init(&sh.o_full[s], 1);
         }
@@ -370,6 +370,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const __grid_con
     auto next_seg = [&](unsigned n) -> const Seg & {
         wait_slot(&sh.seg_full[n % kSegs], (n / kSegs) & 1, &sh.late, p.c.status);
         return sh.seg[n % kSegs];
+    };
+
+    auto arrive = [&](uint64_t *bar) { // a warp's: every lane has fenced what it wrote
+        __syncwarp();
+        if (lane == 0) tqp::mbar_arrive(bar);
     };
 
     if (warp < kSoftWarps) {
@@ -478,7 +483,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const __grid_con
                 together();
                 const float back = *put;
                 tqp::tc_fence_before(); // the last segment's reads of S and O
-                tqp::mbar_arrive(&sh.q_ready[t]);
+                arrive(&sh.q_ready[t]);
 
                 for (int j = 0; j < mine; j++) {
                     const int cs = (tick + j) % kConsts, b0 = half * (kBlocks / 2);
@@ -576,7 +581,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const __grid_con
                         if (seen > (__ffs(bad) - 1) * TQ_KV_BLOCK) L = __int_as_float(0x7fc00000);
                     tmem_wait_st();
                     tqp::tc_fence_before();
-                    tqp::mbar_arrive(&sh.p_ready[t]);
+                    arrive(&sh.p_ready[t]);
                 }
                 together(); // the last w is read
                 *put = L;
@@ -704,8 +709,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const __grid_con
                     *reinterpret_cast<uint4 *>(to + chunk_at(r, c0 + 1 - h)) = h ? a : b;
                 }
                 tqp::fence_proxy_async();
-                tqp::mbar_arrive(&sh.k_full[s]);
-                __syncwarp();
+                arrive(&sh.k_full[s]);
                 if (lane == 0) tqp::mbar_arrive(&sh.code_empty[0]);
                 // ---- values ----
                 wait_slot(&sh.code_full[1], k & 1, &sh.late, p.c.status);
@@ -721,8 +725,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const __grid_con
                     *reinterpret_cast<uint4 *>(to + chunk_at(d, 2 * (blk & 3) + 1)) = b;
                 }
                 tqp::fence_proxy_async();
-                tqp::mbar_arrive(&sh.v_full[s]);
-                __syncwarp();
+                arrive(&sh.v_full[s]);
                 if (lane == 0) tqp::mbar_arrive(&sh.code_empty[1]);
             }
         }
