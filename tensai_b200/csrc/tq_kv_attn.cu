@@ -45,6 +45,7 @@ constexpr int kWide = 4;        // MMA accumulators worked on in turn
 constexpr int kSegCost = 1;     // what a segment costs besides its tiles, in tiles
 constexpr int kMinTiles = 8;    // units per CTA below which fewer CTAs work
 constexpr int kPromptRows = 48; // rows of a sequence above which the prompt kernel takes it
+constexpr double kPromptWork = 512e6; // rows x positions x head size below which it stays off
 constexpr int kDirect = 1024;   // sequences whose lengths are kept in shared memory
 constexpr int kSums = kKvSums;
 constexpr float kPUnit = 16384.f; // p = 1 in float16: its low piece stays normal
@@ -720,7 +721,18 @@ cudaError_t tq_kv_launch_attn(const TqKvView &v, const TqKvAttn &a, int sms, cud
     // More tokens than sequences: some may bring enough rows for the tensor cores.
     // (When others bring none, a long one can hide behind a small count; the
     // kernel here then serves it too, in tiles of 8 or 16 rows.)
-    if (v.hdp <= 128 && (long long)(a.n_tokens - a.n + 1) * p.group > kPromptRows) {
+    // Both sides, 28 query heads of 128 on 4 KV heads, bfloat16, in microseconds
+    // here / there:
+    //   16 sequences of 4096: 28 rows 65 / 73, 42 rows 89 / 72, 98 rows 175 / 77;
+    //   16 sequences of 512 (1.4e6 to 9e6 rows x positions): 28 rows 21 / 37,
+    //   98 rows 42 / 39, 126 rows 47 / 40, 259 rows 74 / 67;
+    //   one of 4096 (at most 15e6): 196 rows 35 / 62, 448 rows 59 / 65, 896 rows 101 / 66.
+    // So the rows decide between them, and the other kernel's fixed time (its
+    // set-up, its second kernel and, for a whole call, this one after it) is worth
+    // it from about 4e6 rows x positions on at a head size of 128. The host knows no
+    // lengths: the table's width stands for them.
+    const double work = (double)a.n_tokens * a.n_q * a.table_cols * v.page * v.hdp;
+    if (v.hdp <= 128 && (long long)(a.n_tokens - a.n + 1) * p.group > kPromptRows && work > kPromptWork) {
         p.rows_cut = kPromptRows;
         const cudaError_t e = tq_kv_launch_prompt(p, sms, st);
         if (e != cudaSuccess) return e;

@@ -332,7 +332,17 @@ def batch(rng, n_kv, hd, page, lens, extra=3, wide=1.0):
     return cache, ref, table
 
 
-def bound(ref_out, mag, qk, top_v, dtype, hd, group, longest, new):
+def widen(table, tokens, n_q, hd, page):
+    """The same table in rows so wide that many rows go to the tensor-memory
+    kernel, whatever the lengths are."""
+    hdp = 64 if hd <= 64 else 128
+    cols = max(table.shape[1], int(512e6 / (tokens * n_q * hdp * page)) + 2)
+    out = np.full((table.shape[0], cols), -1)
+    out[:, :table.shape[1]] = table
+    return out
+
+
+def bound(ref_out, mag, qk, top_v, dtype, hd, group, longest, new, many=False):
     """What the arithmetic allows. Per position: the score's hd products (22 bits
     of q, float32 sums that the tensor cores may truncate: 2^-22 each) move p by
     twice their error; exp2 and the pieces of p 2^-21; 2^-12 where p is one
@@ -344,7 +354,6 @@ def bound(ref_out, mag, qk, top_v, dtype, hd, group, longest, new):
     (after division by the sum of p, which is at least 1). With many rows the
     unit is 2^10 for the largest p times its scale, or up to 2^4 below that:
     2^-25 / 2^10 = 2^-35."""
-    many = max(new, default=0) * group > 48 and hd <= 128  # the tensor-memory kernel
     one = dtype != "f32" and (group > 8 or many)
     rel = 2 * (hd + 16) * 2.0**-22 * qk + (longest + 64) * 2.0**-22 + 2.0**-21 + (2.0**-11 if one else 0)
     half = torch.finfo(DT[dtype]).eps / 2
@@ -356,14 +365,19 @@ def run_attention(cache, ref, table, lens, new, dtype, n_q, rng, scale=None, q_s
     starts = np.concatenate([[0], np.cumsum(new)])
     T, hd = int(starts[-1]), ref.hd
     q = torch.tensor(rng.standard_normal((T + pad, n_q, hd)) * q_scale, device="cuda").to(DT[dtype])
-    out = torch.full_like(q, 7)
-    cache.attention(0, q, cu(starts), cu(lens), cu(table), out=out, scale=scale)
     want, mag, qk, top_v = ref.attention(np_(q), starts, lens, table, hd**-0.5 if scale is None else scale)
-    got = np_(out)
-    assert np.all(got[T:] == 7)
-    tol = bound(want, mag, qk, top_v, dtype, hd, n_q // ref.n_kv, max(lens, default=0), new)
-    err = np.abs(got - want)[:T]
-    assert np.all(err <= tol[:T]), (float(np.max(err - tol[:T])), float(np.max(err)))
+    group = n_q // ref.n_kv
+    for many in (False, True):
+        if many and (hd > 128 or max(new, default=0) * group <= 48):
+            break
+        out = torch.full_like(q, 7)
+        rows = widen(table, T, n_q, hd, ref.page) if many else table
+        cache.attention(0, q, cu(starts), cu(lens), cu(rows), out=out, scale=scale)
+        got = np_(out)
+        assert np.all(got[T:] == 7)
+        tol = bound(want, mag, qk, top_v, dtype, hd, group, max(lens, default=0), new, many)
+        err = np.abs(got - want)[:T]
+        assert np.all(err <= tol[:T]), (many, float(np.max(err - tol[:T])), float(np.max(err)))
     return q, out
 
 
@@ -529,6 +543,111 @@ def test_strided_queries_and_outputs():
             cache.attention(0, rows[:, offset:offset + 384].unflatten(1, (6, 64)), starts, cu(lens), cu(table), out=out)
             assert torch.equal(out, want) and bool((res[:, offset + 384:] == 7).all())
             assert bool((res[:, :offset] == 7).all())
+
+
+def prompts(rng, dtype="f32", group=4):
+    """Three sequences with rows for the tensor-memory kernel, one without."""
+    lens, new = [300, 140, 50, 200], [100, 140, 3, 33]
+    cache, ref, table = batch(rng, 2, 64, 16, lens)
+    starts = np.concatenate([[0], np.cumsum(new)])
+    q = torch.tensor(rng.standard_normal((starts[-1], 2 * group, 64)), device="cuda").to(DT[dtype])
+    return cache, ref, widen(table, len(q), 2 * group, 64, 16), lens, starts, q
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+def test_prompts_nan_stays_where_it_is_seen(dtype):
+    rng = np.random.default_rng(22)
+    cache, ref, table, lens, starts, q = prompts(rng, dtype)
+    with cache:
+        nan = np.float32("nan")
+        good = cache.attention(0, q, cu(starts), cu(lens), cu(table))
+        used = set(table[table >= 0].tolist())
+        for p in range(len(ref.scale[0])):
+            if p not in used:
+                ref.scale[0][p] = ref.scale[1][p] = nan  # nobody's pages
+        ref.scale[1][table[0, 15], 1] = nan  # sequence 0, head 1, positions 240 to 255: its tokens 40 and later
+        ref.scale[0][table[3, 11], 0] = nan  # sequence 3, head 0, positions 176 to 191: its tokens 9 and later
+        cache.load(0, cu(np.arange(len(ref.scale[0]))), *(cu(c, torch.int8) for c in ref.codes),
+                   *(cu(s, torch.float32) for s in ref.scale))
+        want = np.zeros((len(q), 8), bool)
+        want[40:100, 4:] = True
+        want[starts[3] + 9:, :4] = True
+        q[7, 2, 5] = float("inf")  # a query that is not finite spoils its own row
+        want[7, 2] = True
+        out = cache.attention(0, q, cu(starts), cu(lens), cu(table))
+        assert np.array_equal(torch.isnan(out).any(-1).cpu().numpy(), want)
+        clean = torch.tensor(~want, device="cuda")
+        # the rest is as it was but for p's rounding to float16 (2^-12 of the largest value either way, where a
+        # row's largest score is known in another order) and the output's (2^-12 either way)
+        assert float((out.float() - good.float())[clean].abs().max()) <= 4 * 2.0**-12 * float(good.float().abs().max())
+
+
+def test_prompts_bad_pages_and_lengths_are_skipped_and_reported():
+    rng = np.random.default_rng(23)
+    cache, ref, table, lens, starts, q = prompts(rng)
+    with cache:
+        good = cache.attention(0, q, cu(starts), cu(lens), cu(table))
+        others = torch.ones(len(q), dtype=torch.bool, device="cuda")
+        others[100:240] = False
+        for id_ in (-1, len(ref.scale[0]), 2**31 - 1):
+            broken = table.copy()
+            broken[1, 4] = id_
+            out = cache.attention(0, q, cu(starts), cu(lens), cu(broken))
+            assert cache.status() == _lib.TQ_KV_STATUS_PAGE
+            assert torch.equal(out[others], good[others])
+            assert torch.equal(out[100:164], good[100:164])  # they do not see it
+        # without sequence 1 the work is cut elsewhere: the others' sums are joined in another order
+        want, mag, qk, top_v = ref.attention(np_(q), starts, lens, table, 64**-0.5)
+        tol = bound(want, mag, qk, top_v, "f32", 64, 4, 300, [], many=True)
+        for length, bit in ((-1, _lib.TQ_KV_STATUS_LENGTH), (2**30, _lib.TQ_KV_STATUS_TABLE)):
+            out = torch.full_like(q, 9)
+            cache.attention(0, q, cu(starts), cu([300, length, 50, 200]), cu(table), out=out)
+            assert cache.status() == bit and bool((out[100:240] == 9).all())
+            assert np.all((np.abs(np_(out) - want) <= tol)[np_(others)])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_prompts_strided(dtype):
+    rng = np.random.default_rng(24)
+    cache, ref, table, lens, starts, q = prompts(rng, dtype)
+    with cache:
+        args = (cu(starts), cu(lens), cu(table))
+        want = cache.attention(0, q, *args)
+        assert torch.equal(cache.attention(0, q, *args), want)  # the same bits
+        for offset, width in ((0, 1024), (3, 517)):
+            rows = torch.zeros((len(q), width), device="cuda", dtype=q.dtype)
+            rows[:, offset:offset + 512] = q.view(len(q), -1)
+            res = torch.full((len(q), width), 7, device="cuda", dtype=q.dtype)
+            out = res[:, offset:offset + 512].unflatten(1, (8, 64))
+            cache.attention(0, rows[:, offset:offset + 512].unflatten(1, (8, 64)), *args, out=out)
+            assert torch.equal(out, want) and bool((res[:, offset + 512:] == 7).all())
+            assert bool((res[:, :offset] == 7).all())
+
+
+def test_prompts_in_graphs_and_streams_side_by_side():
+    rng = np.random.default_rng(25)
+    cache, ref, table, lens, starts, q = prompts(rng, "bf16")
+    with cache:
+        args = (cu(starts), cu(lens), cu(table))
+        want = cache.attention(0, q, *args)
+        torch.cuda.synchronize()
+        graphs = []
+        for _ in range(2):
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g):
+                out = [cache.attention(0, q, *args) for _ in range(2)]
+            graphs.append((g, out, torch.cuda.Stream()))
+        for _ in range(5):
+            for g, _, st in graphs:
+                with torch.cuda.stream(st):
+                    g.replay()
+            eager = cache.attention(0, q, *args)
+            torch.cuda.synchronize()
+            assert torch.equal(eager, want)
+            assert all(torch.equal(x, want) for _, out, _ in graphs for x in out)
+            for _, out, _ in graphs:
+                for x in out:
+                    x.zero_()
 
 
 def test_offsets_beyond_32_bits():
