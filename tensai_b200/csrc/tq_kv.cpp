@@ -272,7 +272,7 @@ int tq_kv_store_dev(uint64_t cache, int layer, const void *k, const void *v, int
         return tq_fail(TQ_ERR_ARG, "tensai: keys or values not aligned to their type");
     OnDevice on(c->device);
     if (on.err != cudaSuccess) return tq_cuda_fail(on.err, "set device");
-    return done(tq_kv_launch_store(view(*c, layer), k, v, dtype, k_stride, v_stride, slots, n, (cudaStream_t)stream),
+    return done(tq_kv_launch_store(view(*c, layer), k, v, dtype, k_stride, v_stride, slots, n, c->sms, (cudaStream_t)stream),
                 "cache store launch");
 }
 

@@ -54,7 +54,7 @@ cudaError_t tq_kv_launch_plan(int page_shift, int n_pages, unsigned *status, con
 cudaError_t tq_kv_launch_release(int page_shift, int n_pages, unsigned *status, const tq_kv_release_args &a,
                                  cudaStream_t st);
 cudaError_t tq_kv_launch_store(const TqKvView &v, const void *k, const void *val, int dtype, long long k_stride,
-                               long long v_stride, const long long *slots, int n, cudaStream_t st);
+                               long long v_stride, const long long *slots, int n, int sms, cudaStream_t st);
 // Plain [n][page][n_kv][hd] codes and [n][n_kv] scales <-> the listed pages.
 cudaError_t tq_kv_launch_load(const TqKvView &v, const int *pages, int n, const int8_t *k, const int8_t *val,
                               const float *kscale, const float *vscale, cudaStream_t st);

@@ -24,10 +24,11 @@
 
 namespace {
 
-constexpr int kStoreThreads = 256; // or 128 for little pages
+constexpr int kStoreThreads = 1024; // at most; 128 for little pages
 constexpr int kStoreWarps = kStoreThreads / 32;
-constexpr int kMaxPage = 128;
-static_assert(kStoreThreads / 2 >= kMaxPage, "one thread per token of a run");
+constexpr int kMaxPage = 128, kLeastThreads = 128;
+constexpr int kFewTokens = 128; // up to these, runs of one (a decode step) are likelier than a prompt
+static_assert(kLeastThreads >= kMaxPage, "one thread per token of a run");
 constexpr float kRound = 12582912.f; // 1.5 * 2^23: x + kRound holds the integer nearest to x in its low bits
 
 __device__ __forceinline__ float to_f(float x) { return x; }
@@ -109,7 +110,7 @@ template <typename T> __device__ __forceinline__ void eight_at(const T *p, float
 __device__ __forceinline__ unsigned byte_of(unsigned w, int i) { return (w >> (8 * i)) & 0xffu; }
 
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(kStoreThreads, 4) kv_store_kernel(TqKvView c, const T *k, const T *v, long long k_stride,
+__global__ void __launch_bounds__(kStoreThreads, 1) kv_store_kernel(TqKvView c, const T *k, const T *v, long long k_stride,
                                                                  long long v_stride, const long long *slots, int n,
                                                                  int window) {
     extern __shared__ __align__(16) unsigned char store_sm[];
@@ -173,9 +174,7 @@ __global__ void __launch_bounds__(kStoreThreads, 4) kv_store_kernel(TqKvView c, 
         mx = __reduce_max_sync(0xffffffffu, mx);
         if (lane == 0) s_max[warp] = mx;
         __syncthreads();
-#pragma unroll
-        for (int w = 0; w < kStoreWarps; w++)
-            if (w < (int)blockDim.x >> 5) mx = max(mx, s_max[w]);
+        mx = __reduce_max_sync(0xffffffffu, lane < (int)blockDim.x >> 5 ? s_max[lane] : 0u);
         float now = mx < 0x7f800000u ? __fdiv_rn(__uint_as_float(mx), 127.f) : __uint_as_float(0x7fc00000u);
         const float was = held;
         if (off && !(now >= was)) now = now != now ? now : was; // the larger; a NaN stays
@@ -379,8 +378,9 @@ constexpr int kPageThreads = 256;
 
 template <typename T>
 cudaError_t launch_store(const TqKvView &c, const T *k, const T *v, long long ks, long long vs, const long long *slots,
-                         int n, cudaStream_t st) {
-    const size_t smem = (size_t)c.page * c.hd * sizeof(T);
+                         int n, int sms, cudaStream_t st) {
+    const int rows = c.page < n ? c.page : n; // of a run, at most
+    const size_t smem = (size_t)rows * c.hd * sizeof(T);
     static TqDeviceOnce once;
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
@@ -394,10 +394,20 @@ cudaError_t launch_store(const TqKvView &c, const T *k, const T *v, long long ks
             return r;
         });
     if (e != cudaSuccess) return e;
-    // A decode step's tokens are runs of one: a block each. In a prompt most
-    // tokens are not the first of their page, so a block looks through several.
-    const int window = n <= 1024 ? 1 : c.page >= 32 ? 32 : 16;
-    const int threads = c.page * c.hd <= 4096 || n <= 1024 ? kStoreThreads / 2 : kStoreThreads;
+    const long long lines = 2ll * c.n_kv; // (head, side) pairs
+    // Tokens per block, which looks for those that begin a run: a power of two, so that a prompt's
+    // pages fall to the blocks evenly, for a few waves of blocks. (One token a block up to 1024:
+    // 1000 tokens in a row, 8 heads of 128, bfloat16, pages of 64 took 25.7 us, now 12.2.)
+    int window = 1;
+    while (window < (c.page >= 32 ? 32 : 16) && window * 16ll * sms < n * lines) window *= 2;
+    // Threads: 32 elements each of a full page, but 128 at first sight of a decode step, and no more
+    // than the blocks at work (their runs fill shared memory) leave room for. One block an SM: 16000
+    // tokens of 8 float32 heads of 256, pages of 128, 340 us with 256 threads and 171 with 1024.
+    // Three or more: 16000 tokens of 8 bfloat16 heads of 256, 128 us with 256 and 152 with 1024.
+    const long long pages = min(((long long)n / c.page + 1) * lines, (long long)sms * (228 * 1024 / (smem + 2048)));
+    int threads = kLeastThreads;
+    while (threads < kStoreThreads && threads * 32 < rows * c.hd && (threads < 256 ? n > kFewTokens : pages * threads < 768ll * sms))
+        threads *= 2;
     const dim3 grid((n + window - 1) / window, c.n_kv, 2);
     const size_t ax = (uintptr_t)k | (uintptr_t)v | (size_t)(ks * (long long)sizeof(T)) |
                       (size_t)(vs * (long long)sizeof(T)) | (size_t)c.hd * sizeof(T);
@@ -411,13 +421,13 @@ cudaError_t launch_store(const TqKvView &c, const T *k, const T *v, long long ks
 } // namespace
 
 cudaError_t tq_kv_launch_store(const TqKvView &v, const void *k, const void *val, int dtype, long long k_stride,
-                               long long v_stride, const long long *slots, int n, cudaStream_t st) {
+                               long long v_stride, const long long *slots, int n, int sms, cudaStream_t st) {
     if (n == 0) return cudaSuccess;
     if (dtype == TQ_LINEAR_F32)
-        return launch_store(v, (const float *)k, (const float *)val, k_stride, v_stride, slots, n, st);
+        return launch_store(v, (const float *)k, (const float *)val, k_stride, v_stride, slots, n, sms, st);
     if (dtype == TQ_LINEAR_F16)
-        return launch_store(v, (const __half *)k, (const __half *)val, k_stride, v_stride, slots, n, st);
-    return launch_store(v, (const __nv_bfloat16 *)k, (const __nv_bfloat16 *)val, k_stride, v_stride, slots, n, st);
+        return launch_store(v, (const __half *)k, (const __half *)val, k_stride, v_stride, slots, n, sms, st);
+    return launch_store(v, (const __nv_bfloat16 *)k, (const __nv_bfloat16 *)val, k_stride, v_stride, slots, n, sms, st);
 }
 
 cudaError_t tq_kv_launch_load(const TqKvView &v, const int *pages, int n, const int8_t *k, const int8_t *val,
