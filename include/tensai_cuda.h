@@ -441,7 +441,7 @@ TQ_EXPORT int tq_synth_tokens(int *out, int n, int vocab, uint64_t seed);
  * large. Positions live in pages of `page` tokens that any sequence may own;
  * each (page, KV head) holds int8 codes and two float32 scales, one for its
  * keys and one for its values: value = code * scale, |code| <= 127.
- * n_layer, n_kv >= 1; hd (head size) a multiple of 8, at most 256; page 16,
+ * n_layer, n_kv 1 to 65535; hd (head size) a multiple of 8, at most 256; page 16,
  * 32, 64 or 128 tokens; n_pages pages in all, of every layer alike (a page id
  * names the same page in each layer). */
 typedef struct {
@@ -533,7 +533,8 @@ TQ_EXPORT int tq_kv_store_dev(uint64_t cache, int layer, const void *k, const vo
  * starts[i] .. starts[i + 1] - 1, which are the last of its lens[i] positions:
  * row j sees positions 0 .. lens[i] - (starts[i + 1] - starts[i]) + j (its own
  * included) through row i of the table. out = softmax(scale * q . k) v; a row
- * that sees nothing is 0; rows from starts[n] on stay as they were.
+ * that sees nothing is 0; rows from starts[n] on stay as they were. Values of
+ * pages whose value scale is below 2^-92 may count as 0.
  * workspace: tq_kv_attention_workspace bytes of device memory, 16-byte
  * aligned, its first TQ_KV_WORKSPACE_HEAD bytes zero before the first call (each
  * call leaves them zero) and never shared by two calls that may overlap (two
@@ -557,7 +558,8 @@ TQ_EXPORT int tq_kv_attention_dev(uint64_t cache, int layer, const tq_kv_attenti
 /* Pages in and out, for the n page ids in the device array pages: codes as
  * [n][page][n_kv][hd] int8 and scales as [n][n_kv] float32 (load, save), or
  * the values code * scale as [n][page][n_kv][hd] float32 (read). Device
- * memory, asynchronous on stream. load clamps code -128 to -127. */
+ * memory, asynchronous on stream. load clamps code -128 to -127 and takes a
+ * scale that is negative or infinite for NaN. */
 TQ_EXPORT int tq_kv_load_dev(uint64_t cache, int layer, const int *pages, int n, const int8_t *k, const int8_t *v,
                              const float *kscale, const float *vscale, void *stream);
 TQ_EXPORT int tq_kv_save_dev(uint64_t cache, int layer, const int *pages, int n, int8_t *k, int8_t *v, float *kscale,

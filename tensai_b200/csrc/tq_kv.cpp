@@ -7,6 +7,7 @@
 #include <climits>
 #include <cmath>
 #include <cstring>
+#include <initializer_list>
 #include <memory>
 #include <mutex>
 #include <new>
@@ -86,6 +87,16 @@ bool overlap(const void *a, size_t na, const void *b, size_t nb) {
     return na && nb && x < y + nb && y < x + na;
 }
 
+// Whether every pointer is a multiple of `to`, which the kernels' accesses rely on.
+bool aligned(std::initializer_list<const void *> ps, size_t to) {
+    for (const void *p : ps)
+        if ((uintptr_t)p % to) return false;
+    return true;
+}
+int unaligned(const char *what) {
+    return tq_fail(TQ_ERR_ARG, "tensai: %s not aligned to their type", what);
+}
+
 int bad_pages(const char *what, int n) {
     return tq_fail(TQ_ERR_ARG, "tensai: %s of %d pages: null pointer or negative count", what, n);
 }
@@ -99,8 +110,8 @@ extern "C" {
 int tq_kv_create(const tq_kv_config *cfg, uint64_t *cache) {
     if (!cfg || !cache) return tq_fail(TQ_ERR_ARG, "tensai: null pointer argument");
     const tq_kv_config &c = *cfg;
-    if (c.n_layer < 1 || c.n_kv < 1 || c.n_pages < 1 || c.n_kv > 65535)
-        return tq_fail(TQ_ERR_ARG, "tensai: a cache needs layers, KV heads (at most 65535) and pages, got %d, %d, %d",
+    if (c.n_layer < 1 || c.n_kv < 1 || c.n_pages < 1 || c.n_kv > 65535 || c.n_layer > 65535)
+        return tq_fail(TQ_ERR_ARG, "tensai: a cache needs layers, KV heads (at most 65535 each) and pages, got %d, %d, %d",
                        c.n_layer, c.n_kv, c.n_pages);
     if (c.hd < 8 || c.hd > 256 || c.hd % 8)
         return tq_fail(TQ_ERR_ARG, "tensai: cache head size must be a multiple of 8 up to 256, got %d", c.hd);
@@ -202,6 +213,9 @@ int tq_kv_plan_dev(uint64_t cache, const tq_kv_plan_args *args, void *stream) {
     if ((a.n && (!a.cached || !a.added || !a.lens || (!a.table && a.table_cols))) || !a.starts || !a.free_count ||
         !a.free_left || (a.free_cap && !a.free_pages) || (a.slots_cap && !a.slots))
         return tq_fail(TQ_ERR_ARG, "tensai: null pointer argument");
+    if (!aligned({a.cached, a.added, a.table, a.free_pages, a.free_count, a.starts, a.lens, a.free_left}, sizeof(int)) ||
+        !aligned({a.slots}, sizeof(long long)))
+        return unaligned("plan arrays");
     const size_t n4 = sizeof(int) * (size_t)a.n;
     const struct {
         const void *p;
@@ -243,6 +257,8 @@ int tq_kv_release_dev(uint64_t cache, const tq_kv_release_args *args, void *stre
     if ((a.n && (!a.done || !a.lens || (!a.table && a.table_cols))) || !a.free_count || !a.free_left ||
         (a.free_cap && !a.free_pages))
         return tq_fail(TQ_ERR_ARG, "tensai: null pointer argument");
+    if (!aligned({a.done, a.lens, a.table, a.free_pages, a.free_count, a.free_left}, sizeof(int)))
+        return unaligned("release arrays");
     const size_t n4 = sizeof(int) * (size_t)a.n, fb = sizeof(int) * (size_t)a.free_cap,
                  tb = a.n ? sizeof(int) * ((size_t)a.table_stride * (a.n - 1) + a.table_cols) : 0;
     if (overlap(a.lens, n4, a.done, n4) || overlap(a.lens, n4, a.table, tb) || overlap(a.lens, n4, a.free_pages, fb) ||
@@ -268,8 +284,8 @@ int tq_kv_store_dev(uint64_t cache, int layer, const void *k, const void *v, int
     if (n > 1 && (k_stride < row || v_stride < row))
         return tq_fail(TQ_ERR_ARG, "tensai: key and value rows of %lld elements do not fit strides of %lld and %lld",
                        row, k_stride, v_stride);
-    if ((uintptr_t)k % size_of(dtype) || (uintptr_t)v % size_of(dtype))
-        return tq_fail(TQ_ERR_ARG, "tensai: keys or values not aligned to their type");
+    if (!aligned({k, v}, size_of(dtype)) || !aligned({slots}, sizeof(long long)))
+        return unaligned("keys, values or slots");
     OnDevice on(c->device);
     if (on.err != cudaSuccess) return tq_cuda_fail(on.err, "set device");
     return done(tq_kv_launch_store(view(*c, layer), k, v, dtype, k_stride, v_stride, slots, n, c->sms, (cudaStream_t)stream),
@@ -311,8 +327,8 @@ int tq_kv_attention_dev(uint64_t cache, int layer, const tq_kv_attention_args *a
     if (a.n == 0 || a.n_tokens == 0) return TQ_OK;
     if (!a.q || !a.out || !a.starts || !a.lens || (!a.table && a.table_cols) || !a.workspace)
         return tq_fail(TQ_ERR_ARG, "tensai: null pointer argument");
-    if ((uintptr_t)a.q % size_of(a.dtype) || (uintptr_t)a.out % size_of(a.dtype))
-        return tq_fail(TQ_ERR_ARG, "tensai: queries or outputs not aligned to their type");
+    if (!aligned({a.q, a.out}, size_of(a.dtype)) || !aligned({a.starts, a.lens, a.table}, sizeof(int)))
+        return unaligned("queries, outputs, lengths or tables");
     const size_t span_q = size_of(a.dtype) * ((size_t)a.q_stride * (a.n_tokens - 1) + row),
                  span_o = size_of(a.dtype) * ((size_t)a.out_stride * (a.n_tokens - 1) + row);
     if (overlap(a.q, span_q, a.out, span_o)) return tq_fail(TQ_ERR_ARG, "tensai: attention output overlaps its queries");
@@ -320,6 +336,8 @@ int tq_kv_attention_dev(uint64_t cache, int layer, const tq_kv_attention_args *a
     if (a.workspace_bytes < need || (uintptr_t)a.workspace % 16)
         return tq_fail(TQ_ERR_ARG, "tensai: attention needs a 16-byte aligned workspace of %zu bytes, got %zu", need,
                        a.workspace_bytes);
+    if (overlap(a.workspace, need, a.out, span_o) || overlap(a.workspace, need, a.q, span_q))
+        return tq_fail(TQ_ERR_ARG, "tensai: attention workspace overlaps its queries or output");
     OnDevice on(k->device);
     if (on.err != cudaSuccess) return tq_cuda_fail(on.err, "set device");
     const TqKvAttn t = {a.q,      a.out,  a.dtype, a.q_stride,     a.out_stride, a.n_q,   a.n_tokens,
@@ -333,7 +351,8 @@ int tq_kv_load_dev(uint64_t cache, int layer, const int *pages, int n, const int
     auto c = find(cache, &rc);
     if (!c || (rc = check_layer(*c, layer))) return rc;
     if (n < 0 || (n && (!pages || !k || !v || !kscale || !vscale))) return bad_pages("load", n);
-    if ((uintptr_t)k % 4 || (uintptr_t)v % 4) return tq_fail(TQ_ERR_ARG, "tensai: codes must be 4-byte aligned");
+    if (!aligned({k, v}, 4)) return tq_fail(TQ_ERR_ARG, "tensai: codes must be 4-byte aligned");
+    if (!aligned({pages, kscale, vscale}, sizeof(int))) return unaligned("pages or scales");
     OnDevice on(c->device);
     if (on.err != cudaSuccess) return tq_cuda_fail(on.err, "set device");
     return done(tq_kv_launch_load(view(*c, layer), pages, n, k, v, kscale, vscale, (cudaStream_t)stream),
@@ -346,7 +365,8 @@ int tq_kv_save_dev(uint64_t cache, int layer, const int *pages, int n, int8_t *k
     auto c = find(cache, &rc);
     if (!c || (rc = check_layer(*c, layer))) return rc;
     if (n < 0 || (n && (!pages || !k || !v || !kscale || !vscale))) return bad_pages("save", n);
-    if ((uintptr_t)k % 4 || (uintptr_t)v % 4) return tq_fail(TQ_ERR_ARG, "tensai: codes must be 4-byte aligned");
+    if (!aligned({k, v}, 4)) return tq_fail(TQ_ERR_ARG, "tensai: codes must be 4-byte aligned");
+    if (!aligned({pages, kscale, vscale}, sizeof(int))) return unaligned("pages or scales");
     OnDevice on(c->device);
     if (on.err != cudaSuccess) return tq_cuda_fail(on.err, "set device");
     return done(tq_kv_launch_save(view(*c, layer), pages, n, k, v, kscale, vscale, (cudaStream_t)stream),
@@ -358,7 +378,8 @@ int tq_kv_read_dev(uint64_t cache, int layer, const int *pages, int n, float *k,
     auto c = find(cache, &rc);
     if (!c || (rc = check_layer(*c, layer))) return rc;
     if (n < 0 || (n && (!pages || !k || !v))) return bad_pages("read", n);
-    if ((uintptr_t)k % 16 || (uintptr_t)v % 16) return tq_fail(TQ_ERR_ARG, "tensai: values must be 16-byte aligned");
+    if (!aligned({k, v}, 16)) return tq_fail(TQ_ERR_ARG, "tensai: values must be 16-byte aligned");
+    if (!aligned({pages}, sizeof(int))) return unaligned("pages");
     OnDevice on(c->device);
     if (on.err != cudaSuccess) return tq_cuda_fail(on.err, "set device");
     return done(tq_kv_launch_read(view(*c, layer), pages, n, k, v, (cudaStream_t)stream), "cache read launch");

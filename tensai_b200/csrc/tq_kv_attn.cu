@@ -521,7 +521,7 @@ __global__ void __launch_bounds__(32 * warps_of(HDP), 1) kv_attn_kernel(const __
                             const int d = 8 * i + 2 * t;
                             const float y0 = PIECES == 2 ? O[i][0] + O[i][2] : O[i][2 * h];
                             const float y1 = PIECES == 2 ? O[i][1] + O[i][3] : O[i][2 * h + 1];
-                            if (d < p.c.hd) Elem<T>::put2(o + d, y0 * inv, y1 * inv, p.vec, true);
+                            if (d < p.c.hd) Elem<T>::put2(o + d, y0 * inv, y1 * inv, p.vec);
                         }
                     }
                 } else { // to be joined: sums in plain units, m and l
@@ -646,8 +646,8 @@ __global__ void __launch_bounds__(32 * warps_of(HDP), 1) kv_attn_kernel(const __
                 if (d == 0) to[16 * PP + r] = M, to[16 * PP + 16 + r] = L;
             } else if (d < p.c.hd) {
                 const float inv = L == 0.f ? 0.f : 1.f / L;
-                Elem<T>::put2(o + d, A.x * inv, A.y * inv, p.vec, true);
-                Elem<T>::put2(o + d + 2, A.z * inv, A.w * inv, p.vec, true);
+                Elem<T>::put2(o + d, A.x * inv, A.y * inv, p.vec);
+                Elem<T>::put2(o + d + 2, A.z * inv, A.w * inv, p.vec);
             }
         }
     };

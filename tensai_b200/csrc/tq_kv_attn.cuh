@@ -52,68 +52,37 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const unsigned (&a)[4], 
 template <typename T> struct Elem;
 template <> struct Elem<float> {
     static __device__ __forceinline__ float get(const float *p) { return *p; }
-    static __device__ __forceinline__ void put2(float *p, float x, float y, bool vec, bool two) {
+    static __device__ __forceinline__ void put2(float *p, float x, float y, bool vec) {
         if (vec)
             *reinterpret_cast<float2 *>(p) = make_float2(x, y);
         else {
             p[0] = x;
-            if (two) p[1] = y;
+            p[1] = y;
         }
     }
 };
 template <> struct Elem<__half> {
     static __device__ __forceinline__ float get(const __half *p) { return __half2float(*p); }
-    static __device__ __forceinline__ void put2(__half *p, float x, float y, bool vec, bool two) {
+    static __device__ __forceinline__ void put2(__half *p, float x, float y, bool vec) {
         if (vec)
             *reinterpret_cast<__half2 *>(p) = __floats2half2_rn(x, y);
         else {
             p[0] = __float2half_rn(x);
-            if (two) p[1] = __float2half_rn(y);
+            p[1] = __float2half_rn(y);
         }
     }
 };
 template <> struct Elem<__nv_bfloat16> {
     static __device__ __forceinline__ float get(const __nv_bfloat16 *p) { return __bfloat162float(*p); }
-    static __device__ __forceinline__ void put2(__nv_bfloat16 *p, float x, float y, bool vec, bool two) {
+    static __device__ __forceinline__ void put2(__nv_bfloat16 *p, float x, float y, bool vec) {
         if (vec)
             *reinterpret_cast<__nv_bfloat162 *>(p) = __floats2bfloat162_rn(x, y);
         else {
             p[0] = __float2bfloat16_rn(x);
-            if (two) p[1] = __float2bfloat16_rn(y);
+            p[1] = __float2bfloat16_rn(y);
         }
     }
 };
-
-// 8 consecutive elements, widened.
-template <typename T> __device__ __forceinline__ void load8(const T *p, bool vec, float (&x)[8]) {
-    if (vec) {
-        constexpr int E = 16 / sizeof(T);
-#pragma unroll
-        for (int j = 0; j < 8 / E; j++) {
-            const uint4 w = *reinterpret_cast<const uint4 *>(p + j * E);
-            const T *e = reinterpret_cast<const T *>(&w);
-#pragma unroll
-            for (int u = 0; u < E; u++) x[j * E + u] = Elem<T>::get(e + u);
-        }
-    } else {
-#pragma unroll
-        for (int u = 0; u < 8; u++) x[u] = Elem<T>::get(p + u);
-    }
-}
-
-// 8 consecutive elements, rounded.
-template <typename T> __device__ __forceinline__ void store8(T *p, bool vec, const float (&x)[8]) {
-    if (vec) {
-        __align__(16) T e[8];
-#pragma unroll
-        for (int u = 0; u < 8; u += 2) Elem<T>::put2(e + u, x[u], x[u + 1], true, true);
-#pragma unroll
-        for (int j = 0; j < (int)sizeof(e) / 16; j++) reinterpret_cast<uint4 *>(p)[j] = reinterpret_cast<const uint4 *>(e)[j];
-    } else {
-#pragma unroll
-        for (int u = 0; u < 8; u += 2) Elem<T>::put2(p + u, x[u], x[u + 1], false, true);
-    }
-}
 
 // A sequence's lengths, checked: one that cannot be served has no tokens.
 __device__ __forceinline__ Seq seq_at(const TqKvParams &p, const int *starts, const int *lens, int i) {

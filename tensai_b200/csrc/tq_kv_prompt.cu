@@ -19,7 +19,7 @@
 //   P = 2^(w_t - M + 10),  O = sum P v codes,  L = sum_b (sum P) / c_b,
 //   out = O / L:
 // the value scale rides in the exponent at no cost, and P stays below 2^14. A
-// block of value scale 0 counts with c = 1 and zero codes.
+// block of value scale below 2^-92 counts with c = 1 and zero codes.
 //
 // Work: (sequence, KV head, row block) segments laid end to end, each as long as
 // its position tiles and kSegCost units before them (its queries come in and its
@@ -53,6 +53,7 @@ constexpr int kMinUnits = 3;    // units per CTA below which fewer CTAs work
 constexpr float kSlack = 4.f;   // log2 by which w may exceed M
 constexpr float kUnit = 10.f;   // log2 of P at w = M
 constexpr float kLeast = 1e-30f; // least score factor of a block: -inf times it stays -inf
+constexpr float kLeastValue = 0x1p-92f; // value scales below count as 0: 1 / c times 2^14 times 2^20 positions stays finite
 constexpr int kJoinThreads = 256, kJoinRows = 32;
 
 constexpr int stages_of(int hdp, int pieces) { return hdp == 128 && pieces == 2 ? 1 : 2; }
@@ -361,6 +362,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const __grid_con
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     tqp::tc_fence_before();
+    tqp::fence_proxy_async(); // the sums: copies of codes go over them
     __syncthreads();
     tqp::tc_fence_after();
     const uint32_t tmem = sh.tmem;
@@ -616,8 +618,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const __grid_con
                             __align__(16) X e[E];
 #pragma unroll
                             for (int k = 0; k < E; k += 2)
-                                Elem<X>::put2(e + k, __uint_as_float(o[u + k]) * factor, __uint_as_float(o[u + k + 1]) * factor,
-                                              true, true);
+                                Elem<X>::put2(e + k, __uint_as_float(o[u + k]) * factor, __uint_as_float(o[u + k + 1]) * factor, true);
                             *staged(lane, (c + u) / E) = *reinterpret_cast<const uint4 *>(e);
                         }
                     }
@@ -868,14 +869,14 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const __grid_con
         for (unsigned k = 0; b0.some; k++) {
             const Block b2 = ask_page();
             const float2 sc1 = ask_scales(b1);
-            const bool there = b0.id >= 0, some = there && sc.y != 0.f;
+            const bool there = b0.id >= 0, some = there && !(sc.y < kLeastValue);
             const size_t at = there ? kv_block_offset(p.c, b0.id, b0.head, b0.in) : 0;
             const unsigned keys = __ballot_sync(0xffffffffu, there), values = __ballot_sync(0xffffffffu, some);
             const unsigned nan = __ballot_sync(0xffffffffu, there && (sc.x != sc.x || sc.y != sc.y));
             // ---- keys, and the scales ----
             if (k > 0) wait_slot(&sh.code_empty[0], (k - 1) & 1, &sh.late, p.c.status);
             if (lane < kBlocks) {
-                const bool use = there && !(nan >> lane & 1), plain = use && sc.y > 0.f;
+                const bool use = there && !(nan >> lane & 1), plain = use && sc.y >= kLeastValue;
                 sh.f[k % kConsts][lane] = use ? fmaxf(sc.x * mag, kLeast) : kLeast;
                 sh.lv[k % kConsts][lane] = !use ? -INFINITY : plain ? log2f(sc.y) : 0.f;
                 sh.rv[k % kConsts][lane] = !use ? 0.f : plain ? 1.f / sc.y : 1.f;
@@ -948,8 +949,8 @@ __global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const __grid_cons
         const float inv = L == 0.f ? 0.f : 1.f / L;
         const int row = w.rb * kBlockRows + r, tok = row / p.group, hq = w.head * p.group + row - tok * p.group;
         T *o = static_cast<T *>(p.a.out) + (size_t)(w.s.start + tok) * p.a.out_stride + (size_t)hq * p.c.hd + d;
-        Elem<T>::put2(o, A.x * inv, A.y * inv, p.vec, true);
-        Elem<T>::put2(o + 2, A.z * inv, A.w * inv, p.vec, true);
+        Elem<T>::put2(o, A.x * inv, A.y * inv, p.vec);
+        Elem<T>::put2(o + 2, A.z * inv, A.w * inv, p.vec);
     }
 }
 

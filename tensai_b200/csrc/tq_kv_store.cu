@@ -369,9 +369,11 @@ __global__ void kv_load_kernel(TqKvView c, const int *pages, const int8_t *k, co
 #pragma unroll
         for (int j = 0; j < 4; j++) p[j] = make_uint4(x[j][0], x[j][1], x[j][2], x[j][3]);
     }
-    if (threadIdx.x == 0)
-        c.scale[(size_t)id * c.n_kv + head] = make_float2(ks[(size_t)blockIdx.x * c.n_kv + head],
-                                                          vs[(size_t)blockIdx.x * c.n_kv + head]);
+    if (threadIdx.x == 0) { // a scale is a magnitude: a negative or infinite one counts as NaN
+        const float a = ks[(size_t)blockIdx.x * c.n_kv + head], b = vs[(size_t)blockIdx.x * c.n_kv + head];
+        const float nan = __uint_as_float(0x7fc00000u), inf = __uint_as_float(0x7f800000u);
+        c.scale[(size_t)id * c.n_kv + head] = make_float2(a >= 0.f && a < inf ? a : nan, b >= 0.f && b < inf ? b : nan);
+    }
 }
 
 constexpr int kPageThreads = 256;

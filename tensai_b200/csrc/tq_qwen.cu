@@ -1516,6 +1516,11 @@ int tq_qwen_set_cache(uint64_t model, int kind) {
     };
     if (kind == TQ_CACHE_F32) { // the float32 caches first: on failure the 8-bit one stays
         const size_t bytes = sizeof(float) * (size_t)m->c.ctx * m->kvd;
+        try {
+            m->allocs.reserve(m->allocs.size() + 2 * m->L.size());
+        } catch (const std::bad_alloc &) {
+            return tq_fail(TQ_ERR_NOMEM, "tensai: out of host memory for the float32 cache");
+        }
         for (Layer &ly : m->L)
             for (float **p : {&ly.kc, &ly.vc})
                 if (e == cudaSuccess && !*p) e = dalloc(*m, (void **)p, bytes);
@@ -1533,7 +1538,14 @@ int tq_qwen_set_cache(uint64_t model, int kind) {
     uint64_t kv = 0;
     if ((rc = tq_kv_create(&cfg, &kv)) != TQ_OK) return rc;
     m->kv = kv;
-    std::vector<int> ints(kKvTable + 2 * (size_t)m->kv_pages, 0);
+    std::vector<int> ints;
+    try {
+        ints.resize(kKvTable + 2 * (size_t)m->kv_pages);
+        m->allocs.reserve(m->allocs.size() + 3);
+    } catch (const std::bad_alloc &) {
+        drop_kv();
+        return tq_fail(TQ_ERR_NOMEM, "tensai: out of host memory for the 8-bit cache");
+    }
     ints[kKvOne] = 1;
     ints[kKvFree] = m->kv_pages;
     for (int i = 0; i < m->kv_pages; i++) ints[kKvTable + m->kv_pages + i] = m->kv_pages - 1 - i; // page 0 on top

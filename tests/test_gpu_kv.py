@@ -650,6 +650,38 @@ def test_prompts_in_graphs_and_streams_side_by_side():
                     x.zero_()
 
 
+@pytest.mark.parametrize("tiny", [1e-44, 1e-38, 2e-30])
+def test_prompts_of_tiny_values(tiny):
+    """Pages whose value scale is next to nothing beside ordinary ones, and
+    nothing else in a whole sequence: no overflow of its inverse."""
+    rng = np.random.default_rng(26)
+    cache, ref, table, lens, starts, q = prompts(rng)
+    with cache:
+        for i in table[0, 3:9]:
+            ref.scale[1][i] = tiny
+        for i in table[1][table[1] >= 0]:
+            ref.scale[1][i] = tiny
+        cache.load(0, cu(np.arange(len(ref.scale[0]))), *(cu(c, torch.int8) for c in ref.codes),
+                   *(cu(s, torch.float32) for s in ref.scale))
+        want, mag, qk, top_v = ref.attention(np_(q), starts, lens, table, 64**-0.5)
+        tol = bound(want, mag, qk, top_v, "f32", 64, 4, 300, [], many=True)
+        for rows in (table, table[:, :30]):  # the tensor-memory kernel, the small one
+            out = np_(cache.attention(0, q, cu(starts), cu(lens), cu(rows)))
+            # values of scales below 2^-92 may count as 0: 127 * 2^-92 at most
+            assert np.all(np.abs(out - want) <= tol + 127 * 2.0**-92)
+
+
+def test_loaded_scales_are_magnitudes():
+    with KVCache(1, 1, 8, 16, 3) as cache:
+        codes = torch.ones((3, 16, 1, 8), dtype=torch.int8, device="cuda")
+        a, b = cu([[-1.0], [float("inf")], [2.0]], torch.float32), cu([[1.0], [-0.0], [float("-inf")]], torch.float32)
+        cache.load(0, cu([0, 1, 2]), codes, codes, a, b)
+        _, _, ks, vs = cache.save(0, cu([0, 1, 2]))
+        assert torch.isnan(ks[:, 0]).tolist() == [True, True, False] and float(ks[2]) == 2
+        assert torch.isnan(vs[:, 0]).tolist() == [False, False, True] and float(vs[0]) == 1 and float(vs[1]) == 0
+        cache.check()
+
+
 def test_offsets_beyond_32_bits():
     rng = np.random.default_rng(18)
     n_pages, n_kv, hd, page = 40000, 8, 128, 128  # 5.2 GB of keys
@@ -824,6 +856,14 @@ def test_wrong_tensors_are_refused():
             cache.attention(0, x, starts, lens, table, scale=float("nan"))
         with pytest.raises(TensaiError, match="workspace"):
             cache.attention(0, x, starts, lens, table, workspace=torch.zeros(4096, dtype=torch.uint8, device="cuda"))
+        space = cache.workspace()
+        with pytest.raises(TensaiError, match="workspace overlaps"):
+            cache.attention(0, x, starts, lens, table, workspace=space, out=space[4096:4096 + 1536].view(torch.float32).view_as(x))
+        for name, args in (("store", (0, x.data_ptr(), x.data_ptr(), 0, 128, 128, slots.data_ptr() + 4, 3)),
+                           ("store", (0, x.data_ptr() + 2, x.data_ptr(), 0, 128, 128, slots.data_ptr(), 2)),
+                           ("save", (0, lens.data_ptr() + 1, 1, x.data_ptr(), x.data_ptr(), x.data_ptr(), x.data_ptr()))):
+            with pytest.raises(TensaiError, match="not aligned"):
+                _lib.check(getattr(cache._L, f"tq_kv_{name}_dev")(cache._h, *args, 0))
         c, f, k = cu([0]), cu([1, 2]), cu([2])
         with pytest.raises(TensaiError, match="overlap"):
             cache.plan(c, cu([1]), table, f, k, cu([0, 0]), k, slots)
