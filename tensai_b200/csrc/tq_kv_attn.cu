@@ -104,7 +104,7 @@ __global__ void __launch_bounds__(32 * warps_of(HDP), 1) kv_attn_kernel(const __
     const int *starts = direct ? s_starts : p.a.starts, *lens = direct ? s_lens : p.a.lens;
     auto seq_of = [&](int i) {
         Seq s = seq_at(p, starts, lens, i);
-        if (s.nq > p.rows_cut / group) s.nq = 0; // the prompt kernel's
+        if (s.nq > p.tokens_cut) s.nq = 0; // the prompt kernel's
         return s;
     };
     auto tiles_per = [](const Seq &s) { return s.len > kTile ? (s.len + kTile - 1) / kTile : 1; };
@@ -717,7 +717,7 @@ cudaError_t tq_kv_launch_attn(const TqKvView &v, const TqKvAttn &a, int sms, cud
     p.shift_sums = 0;
     while ((a.n >> p.shift_sums) > kSums - 1) p.shift_sums++;
     p.scale2 = a.scale * 1.4426950408889634f;
-    p.rows_cut = INT_MAX;
+    p.tokens_cut = INT_MAX;
     // More tokens than sequences: some may bring enough rows for the tensor cores.
     // (When others bring none, a long one can hide behind a small count; the
     // kernel here then serves it too, in tiles of 8 or 16 rows.)
@@ -733,7 +733,7 @@ cudaError_t tq_kv_launch_attn(const TqKvView &v, const TqKvAttn &a, int sms, cud
     // lengths: the table's width stands for them.
     const double work = (double)a.n_tokens * a.n_q * a.table_cols * v.page * v.hdp;
     if (v.hdp <= 128 && (long long)(a.n_tokens - a.n + 1) * p.group > kPromptRows && work > kPromptWork) {
-        p.rows_cut = kPromptRows;
+        p.tokens_cut = kPromptRows / p.group;
         const cudaError_t e = tq_kv_launch_prompt(p, sms, st);
         if (e != cudaSuccess) return e;
     }

@@ -14,7 +14,7 @@ struct TqKvParams {
     TqKvView c;
     TqKvAttn a;
     int group, vec, shift_sums; // prefix entry = 2^shift_sums sequences
-    int rows_cut;               // sequences of more rows (new tokens x group) are the prompt kernel's
+    int tokens_cut;             // sequences of more new tokens are the prompt kernel's
     float scale2;               // scale * log2(e)
 };
 constexpr int kKvSums = 512;                      // entries of the prefix sums

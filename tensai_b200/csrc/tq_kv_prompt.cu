@@ -1,6 +1,6 @@
 // tq_kv_prompt.cu — attention of many query rows over the paged 8-bit cache on
 // the 5th-generation tensor cores (the formulas are in tq_kv_attn.cu; head sizes
-// up to 128; sequences of more than rows_cut rows).
+// up to 128; sequences of more than tokens_cut new tokens).
 //
 // The rows of a sequence and KV head (new tokens x query heads of the group) are
 // cut into blocks of 256, two tiles A and B of 128 rows, positions into tiles of
@@ -102,7 +102,7 @@ struct Where { // a segment
 
 __device__ __forceinline__ Seq prompt_seq(const Params &p, int i) {
     Seq s = seq_at(p, p.a.starts, p.a.lens, i);
-    if (s.nq <= p.rows_cut / p.group) s.nq = 0; // the other kernel's
+    if (s.nq <= p.tokens_cut) s.nq = 0; // the other kernel's
     return s;
 }
 
