@@ -24,11 +24,21 @@
 // dimension, are one 16-byte read, and q and p are permuted to match. The scores
 // of the MMA's accumulator are the next product's operand in place.
 // All (sequence, KV head, row tile) segments laid end to end, each as long as its
-// tiles and a unit before them for what it costs besides, are cut evenly over the
-// CTAs, then over their warps, wherever the cuts fall (lengths are device data;
+// tiles and, when warps have several, a unit before them for what it costs
+// besides, are cut evenly over the CTAs, then over their warps, wherever the cuts fall (lengths are device data;
 // every CTA makes the same sums). A warp's unfinished segments meet in its
 // CTA, the CTA's in the CTA that arrives last, in a fixed order: results do not
 // depend on timing.
+//
+// Bound. A sequence or two of ordinary length: latency, 9 us for one tile (the
+// launch; lengths, page, codes one after the other from L2; a first pass through
+// the code), 13 us at 2,559 positions with the joins. Many or long ones: the
+// instructions between the copies. 64 sequences of 124,000 positions (28 / 4
+// bfloat16 heads of 128) take 42 us, 3.0 TB/s (46% of the measured copy), 2
+// sequences of 264,000 70 us, 3.9 TB/s (59%). With two warps a scheduler (250
+// registers, and the rings fill shared memory) issue slots are 31% used; waiting
+// for instructions is the largest stall, since a tile's straight code exceeds the
+// instruction caches, then the fixed latency of one instruction after another.
 #include <climits>
 #include <type_traits>
 
@@ -42,10 +52,9 @@ using Params = TqKvParams;
 constexpr int kTile = 64;       // positions per step of a warp
 constexpr int kSlots = 3;       // ring slots per warp
 constexpr int kWide = 4;        // MMA accumulators worked on in turn
-constexpr int kSegCost = 1;     // what a segment costs besides its tiles, in tiles
-constexpr int kMinTiles = 8;    // units per CTA below which fewer CTAs work
+constexpr int kMinTiles = 8;    // units per CTA below which fewer CTAs work: one for each warp
 constexpr int kPromptRows = 48; // rows of a sequence above which the prompt kernel takes it
-constexpr double kPromptWork = 512e6; // rows x positions x head size below which it stays off
+constexpr double kPromptWork = 512e6; // rows x positions x head size up to which it stays off
 constexpr int kDirect = 1024;   // sequences whose lengths are kept in shared memory
 constexpr int kSums = kKvSums;
 constexpr float kPUnit = 16384.f; // p = 1 in float16: its low piece stays normal
@@ -70,7 +79,7 @@ __global__ void __launch_bounds__(32 * warps_of(HDP), 1) kv_attn_kernel(const __
     long long *sums = reinterpret_cast<long long *>(sm + (size_t)NW * kSlots * slot_bytes(HDP));
     int *s_starts = reinterpret_cast<int *>(sums + kSums + 1), *s_lens = s_starts + kDirect + 1;
     __shared__ uint64_t bars[NW][kSlots];
-    __shared__ long long s_scan[NW + 1];
+    __shared__ long long s_scan[NW][2];
     __shared__ long long e_seg[2 * NW], e_end[2 * NW]; // unfinished segments of the warps: first and last tile + 1
     __shared__ int e_row[2 * NW][3];                   // their sequence, KV head, row tile
     __shared__ const float *e_at[2 * NW];              // and where their sums are
@@ -109,57 +118,71 @@ __global__ void __launch_bounds__(32 * warps_of(HDP), 1) kv_attn_kernel(const __
     };
     auto tiles_per = [](const Seq &s) { return s.len > kTile ? (s.len + kTile - 1) / kTile : 1; };
     auto row_tiles = [&](const Seq &s) { return (s.nq * group + R - 1) / R; };
-    auto units_of = [&](int nrt, int tps) { return (long long)nrt * n_kv * (tps + kSegCost); };
+    // A segment counts its tiles and, when the warps have more than one tile each,
+    // another for what it costs besides. 64 sequences of 124,000 positions (28 / 4
+    // heads of 128): 42 us with it, 55 without; 48 short ones: 17 with it, 14 without.
+    int cost;
+    auto units_of = [&](int nrt, int tps) { return (long long)nrt * n_kv * (tps + cost); };
+    auto choose_cost = [&](long long tiles) { cost = tiles > (long long)gridDim.x * NW ? 1 : 0; };
     const int span = 1 << p.shift_sums, entries = (n + span - 1) >> p.shift_sums;
     long long total, lane_sum = 0; // lane_sum: units before sequence `lane`
     if (alone) {
-        long long own = 0;
+        long long segs = 0, tiles = 0;
         if (lane < n) {
             const Seq s = seq_of(lane);
-            own = units_of(row_tiles(s), tiles_per(s));
+            segs = (long long)row_tiles(s) * n_kv;
+            tiles = segs * tiles_per(s);
         }
-        long long inc = own;
+        long long si = segs, ti = tiles;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const long long v = __shfl_up_sync(0xffffffffu, inc, o);
-            if (lane >= o) inc += v;
+            const long long v = __shfl_up_sync(0xffffffffu, si, o), w = __shfl_up_sync(0xffffffffu, ti, o);
+            if (lane >= o) si += v, ti += w;
         }
-        lane_sum = inc - own;
-        total = __shfl_sync(0xffffffffu, inc, 31);
+        total = __shfl_sync(0xffffffffu, ti, 31);
+        choose_cost(total);
+        total += cost * __shfl_sync(0xffffffffu, si, 31);
+        lane_sum = ti - tiles + cost * (si - segs);
     } else { // kSums entries over NT threads
         constexpr int PER = (kSums + NT - 1) / NT;
-        long long own[PER], sum = 0;
+        long long segs[PER], tiles[PER], si = 0, ti = 0;
 #pragma unroll
         for (int u = 0; u < PER; u++) {
             const int e = tid * PER + u;
-            own[u] = 0;
+            segs[u] = tiles[u] = 0;
             for (int i = e << p.shift_sums; e < entries && i < min(n, (e + 1) << p.shift_sums); i++) {
                 const Seq s = seq_of(i);
-                own[u] += units_of(row_tiles(s), tiles_per(s));
+                const long long k = (long long)row_tiles(s) * n_kv;
+                segs[u] += k;
+                tiles[u] += k * tiles_per(s);
             }
-            sum += own[u];
+            si += segs[u];
+            ti += tiles[u];
         }
-        long long inc = sum;
+        const long long own_s = si, own_t = ti;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const long long v = __shfl_up_sync(0xffffffffu, inc, o);
-            if (lane >= o) inc += v;
+            const long long v = __shfl_up_sync(0xffffffffu, si, o), w = __shfl_up_sync(0xffffffffu, ti, o);
+            if (lane >= o) si += v, ti += w;
         }
-        if (lane == 31) s_scan[warp] = inc;
+        if (lane == 31) s_scan[warp][0] = si, s_scan[warp][1] = ti;
         __syncthreads();
-        long long before = 0;
+        long long all_s = 0, before_s = si - own_s, before_t = ti - own_t;
         total = 0;
 #pragma unroll
         for (int w = 0; w < NW; w++) {
-            if (w < warp) before += s_scan[w];
-            total += s_scan[w];
+            const long long a = s_scan[w][0], b = s_scan[w][1];
+            if (w < warp) before_s += a, before_t += b;
+            all_s += a, total += b;
         }
-        before += inc - sum;
+        choose_cost(total);
+        total += cost * all_s;
+        long long before = before_t + cost * before_s;
 #pragma unroll
         for (int u = 0; u < PER; u++) {
             const int e = tid * PER + u;
             if (e <= entries) sums[e] = before;
-            before += own[u];
+            before += tiles[u] + cost * segs[u];
         }
         if (tid == 0 && entries == kSums) sums[kSums] = total;
         __syncthreads();
@@ -196,7 +219,7 @@ __global__ void __launch_bounds__(32 * warps_of(HDP), 1) kv_attn_kernel(const __
         c.pos++;
         if (++c.tile < c.tps) return;
         c.tile = 0;
-        c.pos += kSegCost;
+        c.pos += cost;
         if (++c.rt == c.nrt) {
             c.rt = 0;
             if (++c.head == n_kv) {
@@ -236,11 +259,11 @@ __global__ void __launch_bounds__(32 * warps_of(HDP), 1) kv_attn_kernel(const __
             cur.i++;
             enter(cur);
         }
-        const int per = cur.tps + kSegCost, seg = (int)(rest / per), in = (int)(rest - (long long)seg * per);
+        const int per = cur.tps + cost, seg = (int)(rest / per), in = (int)(rest - (long long)seg * per);
         cur.head = seg / cur.nrt;
         cur.rt = seg - cur.head * cur.nrt;
-        cur.tile = max(0, in - kSegCost);
-        cur.pos = x0 + max(0, kSegCost - in);
+        cur.tile = max(0, in - cost);
+        cur.pos = x0 + max(0, cost - in);
         begin(cur);
     }
     if (x0 < x1 && cur.pos < x1) {
@@ -687,7 +710,9 @@ cudaError_t launch(const Params &p, int sms, cudaStream_t st) {
 
 template <int HDP> cudaError_t launch_hd(const Params &p, int sms, cudaStream_t st) {
     // Two pieces keep float32's precision; a 16-bit query takes one piece when its
-    // rows of one token would not fit the eight that two pieces leave.
+    // rows of one token would not fit the eight that two pieces leave. One piece
+    // everywhere: 16 sequences of 4096, 28 / 4 bfloat16 heads, 2 tokens 35 us in
+    // place of 41, but one of 512 positions 21 in place of 16 and less exact.
     const bool two = p.a.dtype == TQ_LINEAR_F32 || p.group <= 8;
     if (p.a.dtype == TQ_LINEAR_F32) return launch<HDP, 2, float>(p, sms, st);
     if (p.a.dtype == TQ_LINEAR_F16) return two ? launch<HDP, 2, __half>(p, sms, st) : launch<HDP, 1, __half>(p, sms, st);

@@ -13,8 +13,11 @@
 // One launch of one cluster of 1 to 8 blocks: the blocks share the entries and
 // slots evenly, and the cluster's barrier separates all reads of the lengths
 // (into every block's shared memory) and the free count from their updates in
-// place, so a graph that holds the step can be replayed without a copy of either. Bound by latency: the launch,
-// two dependent loads, two scans.
+// place, so a graph that holds the step can be replayed without a copy of either.
+//
+// Bound by latency: the launch, two dependent loads, two scans, the searches.
+// In a graph 8 requests take 3.7 us; 1,024 requests with 54,290 new tokens 10.1
+// us (0.48 MB), with a cluster of four blocks 15.4, with one block 42.8.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 
@@ -225,6 +228,7 @@ cudaError_t set_up() {
 cudaError_t tq_kv_launch_plan(int page_shift, int n_pages, unsigned *status, const tq_kv_plan_args &a, cudaStream_t st) {
     cudaError_t e = set_up();
     if (e != cudaSuccess) return e;
+    // As many blocks as have 2048 requests and slots each (256 each measured the same).
     const long long work = (long long)a.n + a.slots_cap;
     int blocks = 1;
     while (blocks < kMaxCluster && work > (long long)blocks * 2 * kThreads) blocks *= 2;

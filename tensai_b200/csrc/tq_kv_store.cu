@@ -13,8 +13,16 @@
 //   quotient: the product with 1 / scale decides it except within 1e-4 of a
 //   half, where the sign of x - (t + 1/2) scale, exact in one FMA, does. (A
 //   plain float division puts about one value in 10^5 on the wrong side.)
-// Bound by HBM at prompt sizes (element in, byte out), by latency in a decode
-// step.
+// The run is read once, 16 bytes a thread, and stays in shared memory in its own
+// type, because the codes need the maximum first; a value block is written two
+// dimensions a thread, each one 16-byte word.
+//
+// Bound. One token a sequence: latency, 3.8 us for 32 sequences of 4 heads of 128
+// (the slot, the tokens and the scale, the codes of a page that grew). A prompt:
+// 7,096 bfloat16 tokens of 4 heads of 128 take 21 us for 22 MB, half of it issue
+// slots (a code is about 6 instructions), the rest waiting at the two barriers of
+// a block with 1.3 waves of blocks; 16,000 tokens of 8 float32 heads of 128, 164 MB,
+// take 61 us, 2.7 TB/s (41% of the measured copy).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
