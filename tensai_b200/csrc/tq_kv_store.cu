@@ -407,11 +407,13 @@ cudaError_t launch_store(const TqKvView &c, const T *k, const T *v, long long ks
     const long long lines = 2ll * c.n_kv; // (head, side) pairs
     // Tokens per block, which looks for those that begin a run: a power of two, so that a prompt's
     // pages fall to the blocks evenly, for a few waves of blocks. (One token a block up to 1024:
-    // 1000 tokens in a row, 8 heads of 128, bfloat16, pages of 64 took 25.7 us, now 12.2.)
+    // 1000 tokens in a row, 8 heads of 128, bfloat16, pages of 64 took 25.7 us, now 13.1; 300
+    // runs of one 12.3, now 21.)
     int window = 1;
     while (window < (c.page >= 32 ? 32 : 16) && window * 16ll * sms < n * lines) window *= 2;
-    // Threads: 32 elements each of a full page, but 128 at first sight of a decode step, and no more
-    // than the blocks at work (their runs fill shared memory) leave room for. One block an SM: 16000
+    // Threads: 32 elements each of a full page, but 128 for few tokens (100 runs of one, 8 float32
+    // heads of 128: 6.0 us, with 256 threads 8.9; 100 in a row 10.0 and 6.9), and no more than the
+    // blocks at work (their runs fill shared memory) leave room for. One block an SM: 16000
     // tokens of 8 float32 heads of 256, pages of 128, 340 us with 256 threads and 171 with 1024.
     // Three or more: 16000 tokens of 8 bfloat16 heads of 256, 128 us with 256 and 152 with 1024.
     const long long pages = min(((long long)n / c.page + 1) * lines, (long long)sms * (228 * 1024 / (smem + 2048)));
