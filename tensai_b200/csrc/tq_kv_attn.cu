@@ -365,7 +365,8 @@ __global__ void __launch_bounds__(32 * warps_of(HDP), 1) kv_attn_kernel(const __
                         big = fmaxf(big, fabsf(Elem<T>::get(reinterpret_cast<const T *>(&x[kk][0]) + u)));
                 big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
                 big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
-                const float unit = row_scale(big, &row_unit[h]);
+                float unit = row_scale(big, &row_unit[h]);
+                if (p.scale2 < 0.f) unit = -unit; // the block factors stay positive
                 if (live) lim[h] = min(now.s.len, max(0, now.s.len - now.s.nq + tok + 1));
 #pragma unroll
                 for (int kk = 0; kk < KK; kk++)
@@ -431,7 +432,7 @@ __global__ void __launch_bounds__(32 * warps_of(HDP), 1) kv_attn_kernel(const __
             // ---- softmax of the lane's 16 positions (its block), per row ----
             const bool there = sc.x >= 0.f || sc.x != sc.x;
             const bool whole = pos0 + kTile <= least && __all_sync(0xffffffffu, there);
-            const float a = there ? sc.x * p.scale2 : 0.f;
+            const float a = there ? sc.x * fabsf(p.scale2) : 0.f;
             float cmax = there ? sc.y : 0.f;
             cmax = fmaxf(cmax, __shfl_xor_sync(0xffffffffu, cmax, 1));
             cmax = fmaxf(cmax, __shfl_xor_sync(0xffffffffu, cmax, 2));
@@ -444,34 +445,41 @@ __global__ void __launch_bounds__(32 * warps_of(HDP), 1) kv_attn_kernel(const __
             unsigned pf[4][4];
 #pragma unroll
             for (int h = 0; h < H; h++) {
-                const float f = a * row_unit[h];
+                const float af = a * row_unit[h], f = af < kLeast ? kLeast : af; // a NaN stays
                 float v[16], mx = -INFINITY;
                 unsigned hidden = 0; // positions that the row does not see: p = 0 whatever their scales are
 #pragma unroll
                 for (int j = 0; j < 8; j++)
 #pragma unroll
-                    for (int e = 0; e < 2; e++) {
-                        float s = PIECES == 2 ? S[j][e] + S[j][2 + e] : S[j][2 * h + e];
-                        s *= f;
-                        if (!whole && (!there || pos0 + 16 * t + 2 * j + e >= lim[h])) {
-                            s = -INFINITY;
-                            hidden |= 1u << (2 * j + e);
+                    for (int e = 0; e < 2; e++) v[2 * j + e] = PIECES == 2 ? S[j][e] + S[j][2 + e] : S[j][2 * h + e];
+                if (!whole) {
+#pragma unroll
+                    for (int j = 0; j < 16; j++)
+                        if (!there || pos0 + 16 * t + j >= lim[h]) {
+                            v[j] = -INFINITY;
+                            hidden |= 1u << j;
                         }
-                        v[2 * j + e] = s;
-                        mx = fmaxf(mx, s);
-                    }
+                }
+#pragma unroll
+                for (int j = 0; j < 16; j++) mx = fmaxf(mx, v[j]);
+                mx *= f;
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
                 const float m1 = fmaxf(m[h], mx), base = m1 == -INFINITY ? 0.f : m1;
-                const float up = exp2f(m[h] - base);
+                const float up = ex2(m[h] - base);
                 alpha[h] = up * keepC;
                 m[h] = m1;
                 float sum = 0.f;
 #pragma unroll
                 for (int j = 0; j < 16; j++) {
-                    v[j] = exp2f(v[j] - base);
+                    v[j] = ex2(fmaf(v[j], f, -base));
                     sum += v[j];
-                    v[j] = !whole && (hidden >> j & 1) ? 0.f : v[j] * ride;
+                    v[j] *= ride;
+                }
+                if (!whole) {
+#pragma unroll
+                    for (int j = 0; j < 16; j++)
+                        if (hidden >> j & 1) v[j] = 0.f;
                 }
                 l[h] = l[h] * up + sum;
 #pragma unroll

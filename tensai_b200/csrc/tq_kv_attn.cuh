@@ -42,6 +42,14 @@ __device__ __forceinline__ unsigned pack2(float x, float y) {
 }
 __device__ __forceinline__ float2 unpack2(unsigned u) { return __half22float2(*reinterpret_cast<const __half2 *>(&u)); }
 
+// 2^x to about 2^-22 of it; below 2^-126 it is 0, which no sum here can tell.
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+constexpr float kLeast = 1e-30f; // least score factor of a block: -inf times it stays -inf
+
 __device__ __forceinline__ void mma16816(float (&d)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
                  "{%0,%1,%2,%3};"

@@ -63,7 +63,6 @@ constexpr int kSegCost = 2;     // what a segment costs besides its position til
 constexpr int kMinUnits = 3;    // units per CTA below which fewer CTAs work
 constexpr float kSlack = 4.f;   // log2 by which w may exceed M
 constexpr float kUnit = 10.f;   // log2 of P at w = M
-constexpr float kLeast = 1e-30f; // least score factor of a block: -inf times it stays -inf
 constexpr float kLeastValue = 0x1p-92f; // value scales below count as 0: 1 / c times 2^14 times 2^20 positions stays finite
 constexpr int kJoinThreads = 256, kJoinRows = 32;
 
@@ -289,12 +288,6 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
 __device__ __forceinline__ uint64_t desc(uint32_t addr) { return tqp::umma_desc(addr, 16, 1024, 2); }
 // Byte of 16-byte chunk c of row r in such an operand.
 __device__ __forceinline__ uint32_t chunk_at(int r, int c) { return r * 128 + ((c ^ (r & 7)) << 4); }
-
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 
 constexpr int kSegs = 4; // segments known ahead
 

@@ -458,6 +458,16 @@ def test_query_magnitudes(dtype, q_scale):
         run_attention(cache, ref, table, lens, [2, 1], dtype, 3, rng, scale=0.7 if q_scale else 0.0, q_scale=q_scale)
 
 
+@pytest.mark.parametrize("dtype,group", [("f32", 3), ("bf16", 3), ("f16", 12)])
+def test_a_negative_score_factor(dtype, group):
+    rng = np.random.default_rng(27)
+    lens, new = [90, 33, 260], [60, 1, 70]
+    cache, ref, table = batch(rng, 2, 64, 32, lens)
+    with cache:
+        run_attention(cache, ref, table, lens, new, dtype, 2 * group, rng, scale=-0.2)
+        cache.check()
+
+
 def test_zero_scales_and_equal_scores():
     rng = np.random.default_rng(14)
     cache, ref, table = batch(rng, 1, 32, 16, [50])
