@@ -139,8 +139,8 @@ int tq_kv_create(const tq_kv_config *cfg, uint64_t *cache) {
         if (e == cudaSuccess) e = tq_dev_malloc((void **)&l.k, codes);
         if (e == cudaSuccess) e = tq_dev_malloc((void **)&l.v, codes);
         if (e == cudaSuccess) e = tq_dev_malloc((void **)&l.scale, scales);
-        if (e == cudaSuccess) e = cudaMemset(l.k, 0, codes);
-        if (e == cudaSuccess) e = cudaMemset(l.v, 0, codes);
+        if (e == cudaSuccess) e = cudaMemset(l.k, TQ_KV_ZERO, codes);
+        if (e == cudaSuccess) e = cudaMemset(l.v, TQ_KV_ZERO, codes);
         if (e == cudaSuccess) e = cudaMemset(l.scale, 0, scales);
     }
     if (e == cudaSuccess) e = cudaDeviceSynchronize();

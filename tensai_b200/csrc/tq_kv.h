@@ -4,8 +4,9 @@
 // A page holds `page` consecutive positions of one sequence. For each layer,
 // page and KV head it holds page x hdp key codes, page x hdp value codes and
 // one float32 scale for each of the two; a value is code * scale, codes are
-// int8 in [-127, 127]. hdp is the head size rounded up to 64, 128 or 256; the
-// padding holds zero codes. Pages are cut into blocks of 16 positions:
+// integers in [-127, 127], held as the byte code + 128: under the exponent of 1024
+// it is a float16 but for a subtraction. hdp is the head size rounded up to 64, 128
+// or 256; the padding holds zero codes. Pages are cut into blocks of 16 positions:
 //   keys    block = [16 positions][hdp] bytes; the 16-byte chunk c of a row sits
 //           at chunk c ^ ((row & 1) << 2) when hdp >= 128, so that eight lanes
 //           reading four chunks of two adjacent rows hit distinct banks after a
@@ -23,6 +24,8 @@
 #include "../../include/tensai_cuda.h"
 
 #define TQ_KV_BLOCK 16 // positions per block
+#define TQ_KV_ZERO 0x80  // the byte of code 0; a word of four int8 codes ^ TQ_KV_BIAS is what is held, and back
+#define TQ_KV_BIAS 0x80808080u
 
 struct TqKvLayer {
     int8_t *k, *v;

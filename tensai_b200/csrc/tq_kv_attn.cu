@@ -32,10 +32,10 @@
 //
 // Bound. A sequence or two of ordinary length: latency, 9 us for one tile (the
 // launch; lengths, page, codes one after the other from L2; a first pass through
-// the code), 13 us at 2,559 positions with the joins. Many or long ones: the
+// the code), 14 us at 2,559 positions with the joins. Many or long ones: the
 // instructions between the copies. 64 sequences of 124,000 positions (28 / 4
-// bfloat16 heads of 128) take 42 us, 3.0 TB/s (46% of the measured copy), 2
-// sequences of 264,000 70 us, 3.9 TB/s (59%). With two warps a scheduler (250
+// bfloat16 heads of 128) take 41 us, 3.1 TB/s (48% of the measured copy), 2
+// sequences of 264,000 65.5 us, 4.1 TB/s (63%). With two warps a scheduler (250
 // registers, and the rings fill shared memory) issue slots are 31% used; waiting
 // for instructions is the largest stall, since a tile's straight code exceeds the
 // instruction caches, then the fixed latency of one instruction after another.

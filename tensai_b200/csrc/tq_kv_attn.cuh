@@ -26,9 +26,8 @@ struct Seq { // what a sequence's lengths say
     int start, nq, len;
 };
 
-__device__ __forceinline__ void cvt4(unsigned w, unsigned &lo, unsigned &hi) {
+__device__ __forceinline__ void cvt4(unsigned u, unsigned &lo, unsigned &hi) {
     // codes + 128 under the exponent of 1024, then minus 1152: exact
-    const unsigned u = w ^ 0x80808080u;
     const unsigned a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
     const __half2 off = __half2half2(__ushort_as_half(0x6480));
     const __half2 x = __hsub2(*reinterpret_cast<const __half2 *>(&a), off);

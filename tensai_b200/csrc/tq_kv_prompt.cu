@@ -687,7 +687,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const __grid_con
         // a staged word, or zeros for a block that is not there
         auto word_of = [&](int side, int word, unsigned there) {
             const uint4 w = *reinterpret_cast<const uint4 *>(Cs + side * CODES + word * 16);
-            return there >> (word / HDP) & 1 ? w : make_uint4(0, 0, 0, 0);
+            return there >> (word / HDP) & 1 ? w : make_uint4(TQ_KV_BIAS, TQ_KV_BIAS, TQ_KV_BIAS, TQ_KV_BIAS);
         };
         unsigned k = 0;
         for (unsigned n = 0;; n++) {

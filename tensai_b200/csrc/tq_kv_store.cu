@@ -80,9 +80,11 @@ __device__ __forceinline__ unsigned recode(unsigned byte, float was, float now, 
         return (unsigned)(int)rint(__ddiv_rn((double)c * (double)was, (double)now)) & 0xffu;
     return __float_as_uint(v) & 0xffu;
 }
-__device__ __noinline__ unsigned recode4(unsigned w, float was, float now, float ratio) {
-    return recode(w & 0xffu, was, now, ratio) | recode(w >> 8 & 0xffu, was, now, ratio) << 8 |
-           recode(w >> 16 & 0xffu, was, now, ratio) << 16 | recode(w >> 24, was, now, ratio) << 24;
+__device__ __noinline__ unsigned recode4(unsigned held, float was, float now, float ratio) { // four held codes
+    const unsigned w = held ^ TQ_KV_BIAS;
+    return (recode(w & 0xffu, was, now, ratio) | recode(w >> 8 & 0xffu, was, now, ratio) << 8 |
+            recode(w >> 16 & 0xffu, was, now, ratio) << 16 | recode(w >> 24, was, now, ratio) << 24) ^
+           TQ_KV_BIAS;
 }
 
 // e / per and e % per for e = threadIdx.x, + blockDim.x, ..: one division, then steps.
@@ -194,7 +196,7 @@ __global__ void __launch_bounds__(kStoreThreads, 1) kv_store_kernel(TqKvView c, 
             const int chunks = hdp / 16, shift = __ffs(chunks) - 1;
             for (int e = tid + (grew ? 0 : off << shift); e < end << shift; e += blockDim.x) {
                 const int r = e >> shift, d0 = (e - (r << shift)) * 16;
-                if (d0 >= hd) continue; // padding: stays zero
+                if (d0 >= hd) continue; // padding: keeps code 0
                 uint4 *dst = reinterpret_cast<uint4 *>(page + (size_t)(r >> 4) * 16 * hdp +
                                                        kv_key_offset(hdp, r & 15, d0));
                 uint4 w;
@@ -208,8 +210,8 @@ __global__ void __launch_bounds__(kStoreThreads, 1) kv_store_kernel(TqKvView c, 
                     for (int q = 0; q < 4; q += 2) {
                         float y[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
                         if (d0 + 4 * q < hd) eight_at(x + 4 * q, y);
-                        (&w.x)[q] = codes4({y[0], y[1], y[2], y[3]}, now, inv, easy);
-                        (&w.x)[q + 1] = codes4({y[4], y[5], y[6], y[7]}, now, inv, easy);
+                        (&w.x)[q] = codes4({y[0], y[1], y[2], y[3]}, now, inv, easy) ^ TQ_KV_BIAS;
+                        (&w.x)[q + 1] = codes4({y[4], y[5], y[6], y[7]}, now, inv, easy) ^ TQ_KV_BIAS;
                     }
                 }
                 *dst = w;
@@ -248,7 +250,7 @@ __global__ void __launch_bounds__(kStoreThreads, 1) kv_store_kernel(TqKvView c, 
 #pragma unroll
                     for (int h = 0; h < 2; h++) {
                         unsigned &o = (&w[h].x)[q];
-                        o = (o & keep) | (codes4(y[h], now, inv, easy) & ~keep);
+                        o = (o & keep) | ((codes4(y[h], now, inv, easy) ^ TQ_KV_BIAS) & ~keep);
                     }
                 }
                 dst[0] = w[0], dst[1] = w[1];
@@ -308,7 +310,7 @@ __device__ __forceinline__ void page_out(const TqKvView &c, int id, int head, si
         const int r = e / q, d = (e - r * q) * 4;
         const unsigned w =
             *reinterpret_cast<const unsigned *>(pk + (size_t)(r >> 4) * 16 * hdp + kv_key_offset(hdp, r & 15, d));
-        wk(to + (size_t)r * row + d, w);
+        wk(to + (size_t)r * row + d, w ^ TQ_KV_BIAS);
     }
     for (int e = threadIdx.x; side == 1 && e < (c.page >> 4) * q; e += blockDim.x) {
         const int b = e / q, d = (e - b * q) * 4;
@@ -320,7 +322,7 @@ __device__ __forceinline__ void page_out(const TqKvView &c, int id, int head, si
             unsigned t[4];
             transpose4(a, t);
 #pragma unroll
-            for (int j = 0; j < 4; j++) wv(to + (size_t)(16 * b + 4 * u + j) * row + d, t[j]);
+            for (int j = 0; j < 4; j++) wv(to + (size_t)(16 * b + 4 * u + j) * row + d, t[j] ^ TQ_KV_BIAS);
         }
     }
 }
@@ -345,8 +347,8 @@ __global__ void kv_save_kernel(TqKvView c, const int *pages, int8_t *k, int8_t *
     }
 }
 
-// -128 is no code of the cache: -127 in its place.
-__device__ __forceinline__ unsigned no_min(unsigned w) { return __vmaxs4(w, 0x81818181u); }
+// Four int8 codes as they are held. -128 is no code of the cache: -127 in its place.
+__device__ __forceinline__ unsigned held4(unsigned w) { return __vmaxs4(w, 0x81818181u) ^ TQ_KV_BIAS; }
 
 __global__ void kv_load_kernel(TqKvView c, const int *pages, const int8_t *k, const int8_t *v, const float *ks,
                                const float *vs) {
@@ -358,7 +360,7 @@ __global__ void kv_load_kernel(TqKvView c, const int *pages, const int8_t *k, co
     for (int e = threadIdx.x; e < c.page * q; e += blockDim.x) {
         const int r = e / q, d = (e - r * q) * 4;
         const unsigned w = *reinterpret_cast<const unsigned *>(k + from + (size_t)r * row + d);
-        *reinterpret_cast<unsigned *>(pk + (size_t)(r >> 4) * 16 * hdp + kv_key_offset(hdp, r & 15, d)) = no_min(w);
+        *reinterpret_cast<unsigned *>(pk + (size_t)(r >> 4) * 16 * hdp + kv_key_offset(hdp, r & 15, d)) = held4(w);
     }
     for (int e = threadIdx.x; e < (c.page >> 4) * q; e += blockDim.x) {
         const int b = e / q, d = (e - b * q) * 4;
@@ -368,7 +370,7 @@ __global__ void kv_load_kernel(TqKvView c, const int *pages, const int8_t *k, co
             unsigned a[4], t[4];
 #pragma unroll
             for (int j = 0; j < 4; j++)
-                a[j] = no_min(*reinterpret_cast<const unsigned *>(v + from + (size_t)(16 * b + 4 * u + j) * row + d));
+                a[j] = held4(*reinterpret_cast<const unsigned *>(v + from + (size_t)(16 * b + 4 * u + j) * row + d));
             transpose4(a, t);
 #pragma unroll
             for (int j = 0; j < 4; j++) x[j][u] = t[j];
