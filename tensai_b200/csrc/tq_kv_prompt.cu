@@ -66,10 +66,11 @@ constexpr float kUnit = 10.f;   // log2 of P at w = M
 constexpr float kLeastValue = 0x1p-92f; // value scales below count as 0: 1 / c times 2^14 times 2^20 positions stays finite
 constexpr int kJoinThreads = 256, kJoinRows = 32;
 
+constexpr size_t kSharedRoom = 3 * 1024; // struct Shared, behind the operands
 constexpr int stages_of(int hdp, int pieces) { return hdp == 128 && pieces == 2 ? 1 : 2; }
 constexpr size_t operand_bytes(int hdp) { return (size_t)kPos * hdp * 2; } // a K or V tile, or a piece of a Q tile
 constexpr size_t smem_bytes(int hdp, int pieces) {
-    return 3072 + operand_bytes(hdp) * (2 * pieces + 2 * stages_of(hdp, pieces) + 1); // struct Shared; the staged codes are one more
+    return kSharedRoom + operand_bytes(hdp) * (2 * pieces + 2 * stages_of(hdp, pieces) + 1); // the staged codes are one more
 }
 constexpr size_t partial_floats(int hdp) { return (size_t)kBlockRows * (hdp + 2); }
 
@@ -320,7 +321,7 @@ struct Shared { // behind the operands
     uint32_t tmem;
     volatile int late;
 };
-static_assert(sizeof(Shared) <= 3072, "the room behind the operands");
+static_assert(sizeof(Shared) <= kSharedRoom, "the room behind the operands");
 
 template <int HDP, int PIECES, typename T>
 __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const __grid_constant__ Params p) {
