@@ -191,6 +191,32 @@ def test_store_bit_for_bit(dtype, n_kv, hd, page, runs):
         codes_equal(cache, untouched, np.arange(n_pages), 0)
 
 
+@pytest.mark.parametrize("dtype,n_kv,hd,page,T", [("f32", 12, 8, 32, 4000), ("bf16", 12, 16, 16, 2500), ("f32", 2, 256, 128, 700),
+                                                  ("f16", 2, 256, 128, 130)])
+def test_store_of_many_runs(dtype, n_kv, hd, page, T):
+    """Runs of all lengths that begin anywhere in a page, skipped tokens between
+    them: blocks that look for several runs, and blocks of 1,024 threads."""
+    rng = np.random.default_rng(T)
+    slots, at = [], 0
+    while len(slots) < T:
+        if rng.random() < 0.2:
+            slots += [-1] * int(rng.integers(1, 4))
+        off = int(rng.integers(0, page))
+        run = int(rng.integers(1, 3)) if rng.random() < 0.5 else int(rng.integers(1, 3 * page))
+        for p in range(off, off + run):
+            slots.append((at + p // page) * page + p % page)
+        at += (off + run - 1) // page + 1
+    slots, n_pages = slots[:T], at
+    with KVCache(1, n_kv, hd, page, n_pages) as cache:
+        ref = kvref.Ref(n_kv, hd, page, n_pages)
+        random_pages(cache, ref, rng)
+        k, v = (torch.tensor(rng.standard_normal((T, n_kv, hd)) * s, device="cuda").to(DT[dtype]) for s in (3, 0.1))
+        cache.store(0, k, v, i64(slots))
+        cache.check()
+        ref.store(np_(k), np_(v), slots)
+        codes_equal(cache, ref, np.arange(n_pages))
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_token_by_token_appends(dtype):
     """A page filled one token at a time, its scale growing on the way."""
@@ -432,6 +458,19 @@ def test_many_sequences(n):
     cache, ref, table = batch(rng, 1, 16, 16, lens)
     with cache:
         run_attention(cache, ref, table, lens, list(rng.integers(0, 3, n)), "f32", 2, rng)
+        cache.check()
+
+
+@pytest.mark.parametrize("n", [40, 600, 1300])
+def test_many_sequences_some_with_many_rows(n):
+    rng = np.random.default_rng(n)
+    lens = list(rng.integers(0, 90, n))
+    new = list(rng.integers(0, 3, n))
+    for i in range(3, n, 17):  # some as long as their sequence, or a row short of the other kernel's
+        new[i] = min(int(lens[i]), [30, 24, 25, 90][i % 4])
+    cache, ref, table = batch(rng, 1, 16, 16, lens)
+    with cache:
+        run_attention(cache, ref, table, lens, new, "bf16", 2, rng)
         cache.check()
 
 
