@@ -445,9 +445,11 @@ __global__ void __launch_bounds__(32 * warps_of(HDP), 1) kv_attn_kernel(const __
             unsigned pf[4][4];
 #pragma unroll
             for (int h = 0; h < H; h++) {
-                const float af = a * row_unit[h], f = af < kLeast ? kLeast : af; // a NaN stays
+                // a block that the row sees nothing of has the factors of one that is not there: 0 times a NaN is no 0
+                const bool none = !there || pos0 + 16 * t >= lim[h];
+                const float af = none ? 0.f : a * row_unit[h], f = af < kLeast ? kLeast : af; // a NaN stays
+                const float r = none ? 0.f : ride;
                 float v[16], mx = -INFINITY;
-                unsigned hidden = 0; // positions that the row does not see: p = 0 whatever their scales are
 #pragma unroll
                 for (int j = 0; j < 8; j++)
 #pragma unroll
@@ -455,10 +457,7 @@ __global__ void __launch_bounds__(32 * warps_of(HDP), 1) kv_attn_kernel(const __
                 if (!whole) {
 #pragma unroll
                     for (int j = 0; j < 16; j++)
-                        if (!there || pos0 + 16 * t + j >= lim[h]) {
-                            v[j] = -INFINITY;
-                            hidden |= 1u << j;
-                        }
+                        if (!there || pos0 + 16 * t + j >= lim[h]) v[j] = -INFINITY;
                 }
 #pragma unroll
                 for (int j = 0; j < 16; j++) mx = fmaxf(mx, v[j]);
@@ -474,12 +473,7 @@ __global__ void __launch_bounds__(32 * warps_of(HDP), 1) kv_attn_kernel(const __
                 for (int j = 0; j < 16; j++) {
                     v[j] = ex2(fmaf(v[j], f, -base));
                     sum += v[j];
-                    v[j] *= ride;
-                }
-                if (!whole) {
-#pragma unroll
-                    for (int j = 0; j < 16; j++)
-                        if (hidden >> j & 1) v[j] = 0.f;
+                    v[j] *= r;
                 }
                 l[h] = l[h] * up + sum;
 #pragma unroll
