@@ -527,6 +527,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const __grid_con
                         }
                         tmem_wait_st();
                     }
+                    // a block's factor of the row's scores; never 0, for -inf times it is to stay -inf
+                    auto factor = [&](int b) { return fmaxf(sh.f[cs][b0 + b] * back, kLeast); };
                     // ---- M ----
                     float top = -INFINITY;
                     over([&](int b, const uint32_t (&v)[16]) {
@@ -534,7 +536,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const __grid_con
 #pragma unroll
                         for (int u = 1; u < 15; u += 2) mx = max3(mx, __uint_as_float(v[u]), __uint_as_float(v[u + 1]));
                         mx = fmaxf(mx, __uint_as_float(v[15]));
-                        top = fmaxf(top, fmaf(mx, sh.f[cs][b0 + b] * back, sh.lv[cs][b0 + b]));
+                        top = fmaxf(top, fmaf(mx, factor(b), sh.lv[cs][b0 + b]));
                     });
                     *put = top;
                     together();
@@ -563,7 +565,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const __grid_con
                     const float use = M == -INFINITY ? 0.f : M - kUnit;
                     over([&](int b, const uint32_t (&v)[16]) {
                         uint32_t y[16];
-                        const float fb = sh.f[cs][b0 + b] * back, ob = sh.lv[cs][b0 + b] - use;
+                        const float fb = factor(b), ob = sh.lv[cs][b0 + b] - use;
                         float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
                         for (int u = 0; u < 16; u += 2) {
@@ -882,7 +884,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const __grid_con
             if (k > 0) wait_slot(&sh.code_empty[0], (k - 1) & 1, &sh.late, p.c.status);
             if (lane < kBlocks) {
                 const bool use = there && !(nan >> lane & 1), plain = use && sc.y >= kLeastValue;
-                sh.f[k % kConsts][lane] = use ? fmaxf(sc.x * mag, kLeast) : kLeast;
+                sh.f[k % kConsts][lane] = use ? sc.x * mag : 0.f;
                 sh.lv[k % kConsts][lane] = !use ? -INFINITY : plain ? log2f(sc.y) : 0.f;
                 sh.rv[k % kConsts][lane] = !use ? 0.f : plain ? 1.f / sc.y : 1.f;
             }
