@@ -533,8 +533,9 @@ TQ_EXPORT int tq_kv_store_dev(uint64_t cache, int layer, const void *k, const vo
  * starts[i] .. starts[i + 1] - 1, which are the last of its lens[i] positions:
  * row j sees positions 0 .. lens[i] - (starts[i + 1] - starts[i]) + j (its own
  * included) through row i of the table. out = softmax(scale * q . k) v; a row
- * that sees nothing is 0; rows from starts[n] on stay as they were. Values of
- * pages whose value scale is below 2^-92 may count as 0.
+ * that sees nothing is 0; rows from starts[n] on stay as they were. The value
+ * scales of the pages that a row sees may be up to 2^100 apart; values of a
+ * scale below 2^-80 may count as 0.
  * workspace: tq_kv_attention_workspace bytes of device memory, 16-byte
  * aligned, its first TQ_KV_WORKSPACE_HEAD bytes zero before the first call (each
  * call leaves them zero) and never shared by two calls that may overlap (two

@@ -3,7 +3,7 @@
 //
 // For a query row q and the positions t that it sees, with codes k_t, v_t and
 // the scales a_b, c_b of the block b that holds t:
-//   s_t = (q . k_t) a_b scale log2(e),  m = max s_t,  p_t = 2^(s_t - m),
+//   s_t = (q . k_t) a_b scale log2(e),  p_t = 2^(s_t - max s_t),
 //   out = sum_t p_t c_b v_t / sum_t p_t,
 // in one pass over the positions with a running m, sum and accumulator.
 //
@@ -14,8 +14,10 @@
 // products for float32 queries, at no cost while a KV head has at most 8 rows.
 // With PIECES = 1 a 16-bit q is one float16 (exact: the row is scaled by a power
 // of two first) and p is rounded to 11 bits, below the output's own rounding.
-// c_b rides on p: p_t c_b / C with C the largest c_b so far (a running value
-// like m), so that it stays in float16's range; the sum of p itself is float32.
+// The value scale c_b = 2^e_b x mantissa goes with the weights, so that what a row
+// gives no weight, or does not see, costs the rest no bits: m is a power of two at
+// or above 2^(s_t + e_b), p_t = 2^(s_t + e_b - m), the mantissa rides on p in
+// float16's range, and the sum is of p_t 2^-e_b, float32. Both powers are exact.
 //
 // Work. A warp takes 64 positions at a time: keys and values come by bulk copies
 // of 16-position blocks into its own ring of three slots (k, v, k, ..), two of
@@ -34,8 +36,8 @@
 // launch; lengths, page, codes one after the other from L2; a first pass through
 // the code), 14 us at 2,559 positions with the joins. Many or long ones: the
 // instructions between the copies. 64 sequences of 124,000 positions (28 / 4
-// bfloat16 heads of 128) take 41 us, 3.1 TB/s (48% of the measured copy), 2
-// sequences of 264,000 65.5 us, 4.1 TB/s (63%). With two warps a scheduler (250
+// bfloat16 heads of 128) take 39.5 us, 3.2 TB/s (50% of the measured copy), 2
+// sequences of 264,000 64 us, 4.2 TB/s (65%). With two warps a scheduler (248
 // registers, and the rings fill shared memory) issue slots are 31% used; waiting
 // for instructions is the largest stall, since a tile's straight code exceeds the
 // instruction caches, then the fixed latency of one instruction after another.
@@ -57,7 +59,7 @@ constexpr int kPromptRows = 48; // rows of a sequence above which the prompt ker
 constexpr double kPromptWork = 512e6; // rows x positions x head size up to which it stays off
 constexpr int kDirect = 1024;   // sequences whose lengths are kept in shared memory
 constexpr int kSums = kKvSums;
-constexpr float kPUnit = 16384.f; // p = 1 in float16: its low piece stays normal
+constexpr float kPUnit = 16384.f; // p = 1 in float16: times a mantissa it stays below 2^15, its low piece normal
 constexpr size_t kHead = kKvHead;
 constexpr int kMaxGrid = kHead / sizeof(unsigned);
 
@@ -314,7 +316,7 @@ __global__ void __launch_bounds__(32 * warps_of(HDP), 1) kv_attn_kernel(const __
 
         unsigned qf[KK][4][4];
         float O[NI][4];
-        float m[2], l[2], C = 0.f, row_unit[2];
+        float m[2], l[2], row_unit[2];
         int lim[2], least = 0;
         long long seg_from = 0;
         auto start = [&](const Cursor &now) { // a segment: its queries, and nothing seen yet
@@ -327,7 +329,6 @@ __global__ void __launch_bounds__(32 * warps_of(HDP), 1) kv_attn_kernel(const __
                 row_unit[h] = 1.f;
                 lim[h] = now.s.len;
             }
-            C = 0.f;
 #pragma unroll
             for (int i = 0; i < NI; i++) O[i][0] = O[i][1] = O[i][2] = O[i][3] = 0.f;
 #pragma unroll
@@ -432,14 +433,14 @@ __global__ void __launch_bounds__(32 * warps_of(HDP), 1) kv_attn_kernel(const __
             // ---- softmax of the lane's 16 positions (its block), per row ----
             const bool there = sc.x >= 0.f || sc.x != sc.x;
             const bool whole = pos0 + kTile <= least && __all_sync(0xffffffffu, there);
-            const float a = there ? sc.x * fabsf(p.scale2) : 0.f;
-            float cmax = there ? sc.y : 0.f;
-            cmax = fmaxf(cmax, __shfl_xor_sync(0xffffffffu, cmax, 1));
-            cmax = fmaxf(cmax, __shfl_xor_sync(0xffffffffu, cmax, 2));
-            const float C1 = fmaxf(C, cmax);
-            const float keepC = C1 > 0.f ? C / C1 : 1.f;
-            const float ride = C1 > 0.f ? (there ? sc.y : 0.f) / C1 * kPUnit : (there ? sc.y : 0.f);
-            C = C1;
+            const float a = there ? sc.x * fabsf(p.scale2) : 0.f, c = there ? sc.y : 0.f;
+            // c = 2^lift x its mantissa, which rides on p in units of kPUnit; drop = 2^-lift
+            const bool valued = c >= kLeastValue;
+            const unsigned power = __float_as_uint(valued ? c : kNoValue) & 0x7f800000u;
+            const float lift = (float)((int)(power >> 23) - 127);
+            const float drop = __uint_as_float(max(0x7f000000u - power, 0x00400000u)); // 2^-127 has no exponent
+            const float ride = valued ? kPUnit * __uint_as_float((__float_as_uint(c) & 0x007fffffu) | 0x3f800000u)
+                                      : c != c ? c : 0.f;
             constexpr int H = 3 - PIECES;
             float alpha[2];
             unsigned pf[4][4];
@@ -461,21 +462,20 @@ __global__ void __launch_bounds__(32 * warps_of(HDP), 1) kv_attn_kernel(const __
                 }
 #pragma unroll
                 for (int j = 0; j < 16; j++) mx = fmaxf(mx, v[j]);
-                mx *= f;
+                mx = fmaf(mx, f, lift);
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-                const float m1 = fmaxf(m[h], mx), base = m1 == -INFINITY ? 0.f : m1;
-                const float up = ex2(m[h] - base);
-                alpha[h] = up * keepC;
+                const float m1 = fmaxf(m[h], ceilf(mx)), base = m1 == -INFINITY ? 0.f : m1, off = lift - base;
+                alpha[h] = ex2(m[h] - base);
                 m[h] = m1;
                 float sum = 0.f;
 #pragma unroll
                 for (int j = 0; j < 16; j++) {
-                    v[j] = ex2(fmaf(v[j], f, -base));
+                    v[j] = ex2(fmaf(v[j], f, off));
                     sum += v[j];
                     v[j] *= r;
                 }
-                l[h] = l[h] * up + sum;
+                l[h] = fmaf(sum, drop, l[h] * alpha[h]);
 #pragma unroll
                 for (int u = 0; u < 4; u++)
 #pragma unroll
@@ -524,7 +524,7 @@ __global__ void __launch_bounds__(32 * warps_of(HDP), 1) kv_attn_kernel(const __
             // ---- the segment's end, or the warp's ----
             const bool ends = now.tile + 1 == now.tps;
             if (ends || !more) {
-                const float unit = C / kPUnit;
+                constexpr float unit = 1.f / kPUnit;
 #pragma unroll
                 for (int h = 0; h < H; h++) {
                     l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);

@@ -48,6 +48,8 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 constexpr float kLeast = 1e-30f; // least score factor of a block: -inf times it stays -inf
+constexpr float kLeastValue = 0x1p-92f; // value scales below count as 0: the sums that hold their inverse stay finite
+constexpr float kNoValue = 0x1p-60f;    // what such a scale, of no values, counts as beside others
 
 __device__ __forceinline__ void mma16816(float (&d)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "

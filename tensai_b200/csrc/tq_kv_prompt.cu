@@ -63,7 +63,6 @@ constexpr int kSegCost = 2;     // what a segment costs besides its position til
 constexpr int kMinUnits = 3;    // units per CTA below which fewer CTAs work
 constexpr float kSlack = 4.f;   // log2 by which w may exceed M
 constexpr float kUnit = 10.f;   // log2 of P at w = M
-constexpr float kLeastValue = 0x1p-92f; // value scales below count as 0: 1 / c times 2^14 times 2^20 positions stays finite
 constexpr int kJoinThreads = 256, kJoinRows = 32;
 
 constexpr size_t kSharedRoom = 3 * 1024; // struct Shared, behind the operands

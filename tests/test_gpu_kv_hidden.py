@@ -75,3 +75,40 @@ def test_a_stored_key_that_is_not_finite_spoils_later_rows_alone(dtype, group):
         out = cache.attention(0, q, cu([0, 2]), cu([17]), cu([[0, 1]]))
         assert bool(torch.isfinite(out[0]).all()) and bool(torch.isnan(out[1]).all())
         compare(cache, ref, q, np.array([0, 2]), [17], np.array([[0, 1]]), dtype)
+
+
+@pytest.mark.parametrize("dtype,group", KINDS)
+@pytest.mark.parametrize("far", [2.0**30, 2.0**60])
+def test_large_values_behind_a_row_cost_it_nothing(dtype, group, far):
+    """The last token alone sees a page whose values are `far` times the others'."""
+    rng = np.random.default_rng(33)
+    lens, new, page = [33, 65], [3, 2], 16
+    cache, ref, table = batch(rng, 1, 64, page, lens)
+    with cache:
+        ref.scale[1][table[0, 2]] *= np.float32(far)
+        ref.scale[1][table[1, 4]] *= np.float32(far)
+        load(cache, ref)
+        q = torch.tensor(rng.standard_normal((5, group, 64)), device="cuda").to(DT[dtype])
+        rows = [0, 1, 3] if dtype == "f16" else None  # the others are beyond float16
+        compare(cache, ref, q, np.array([0, 3, 5]), lens, table, dtype, rows)
+        cache.check()
+
+
+@pytest.mark.parametrize("dtype,group", KINDS)
+@pytest.mark.parametrize("many", [False, True])
+def test_large_values_of_no_weight_cost_nothing(dtype, group, many):
+    """A page that every row sees, of values 2^45 times the others', whose keys
+    point away from the queries: scores about 300 below the others'."""
+    rng = np.random.default_rng(34)
+    new, page = (60 if many else 2), 16
+    lens = [100]
+    cache, ref, table = batch(rng, 1, 64, page, lens)
+    with cache:
+        u = rng.choice([-1.0, 1.0], 64)
+        ref.codes[0][table[0, 1], :, 0] = -127 * u
+        ref.scale[0][table[0, 1]] = 300 / (127 * 8)  # times 64 dimensions, times 64^-0.5
+        ref.scale[1][table[0, 1]] *= np.float32(2.0**45)
+        load(cache, ref)
+        q = torch.tensor(u + 0.1 * rng.standard_normal((new, group, 64)), device="cuda").to(DT[dtype])
+        compare(cache, ref, q, np.array([0, new]), lens, table, dtype, many=many)
+        cache.check()
