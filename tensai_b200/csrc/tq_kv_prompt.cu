@@ -19,7 +19,8 @@
 //   P = 2^(w_t - M + 10),  O = sum P v codes,  L = sum_b (sum P) / c_b,
 //   out = O / L:
 // the value scale rides in the exponent at no cost, and P stays below 2^14. A
-// block of value scale below 2^-92 counts with c = 1 and zero codes.
+// block of value scale below 2^-92 counts with c = 2^-60 and zero codes: low enough
+// for the bits of what has values, high enough for its own share of L.
 //
 // Work: (sequence, KV head, row block) segments laid end to end, each as long as
 // its position tiles and kSegCost units before them (its queries come in and its
@@ -884,8 +885,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const __grid_con
             if (lane < kBlocks) {
                 const bool use = there && !(nan >> lane & 1), plain = use && sc.y >= kLeastValue;
                 sh.f[k % kConsts][lane] = use ? sc.x * mag : 0.f;
-                sh.lv[k % kConsts][lane] = !use ? -INFINITY : plain ? log2f(sc.y) : 0.f;
-                sh.rv[k % kConsts][lane] = !use ? 0.f : plain ? 1.f / sc.y : 1.f;
+                sh.lv[k % kConsts][lane] = !use ? -INFINITY : log2f(plain ? sc.y : kNoValue);
+                sh.rv[k % kConsts][lane] = !use ? 0.f : 1.f / (plain ? sc.y : kNoValue);
             }
             if (lane == 0) sh.live[0] = keys, sh.poison[k % kConsts] = nan;
             __syncwarp();

@@ -112,3 +112,24 @@ def test_large_values_of_no_weight_cost_nothing(dtype, group, many):
         q = torch.tensor(u + 0.1 * rng.standard_normal((new, group, 64)), device="cuda").to(DT[dtype])
         compare(cache, ref, q, np.array([0, new]), lens, table, dtype, many=many)
         cache.check()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("many", [False, True])
+@pytest.mark.parametrize("small", [2.0**-20, 2.0**-40, 2.0**-60])
+def test_small_values_beside_pages_of_zeros(dtype, many, small):
+    """Every other page holds zeros, the rest values of `small`: the outputs are
+    as exact as if the zeros were not there."""
+    rng = np.random.default_rng(35)
+    lens, new = [300, 77], ([100, 60] if many else [2, 1])
+    cache, ref, table = batch(rng, 2, 64, 16, lens)
+    with cache:
+        for i in range(2):
+            ids = table[i][table[i] >= 0]
+            ref.scale[1][ids[::2]] = 0
+            ref.scale[1][ids[1::2]] = np.float32(small)
+        load(cache, ref)
+        starts = np.concatenate([[0], np.cumsum(new)])
+        q = torch.tensor(rng.standard_normal((starts[-1], 6, 64)), device="cuda").to(DT[dtype])
+        compare(cache, ref, q, starts, lens, table, dtype, many=many)
+        cache.check()
