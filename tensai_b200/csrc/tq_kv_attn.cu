@@ -13,7 +13,8 @@
 // + lo (and p likewise), each a float16, which keeps 22 bits of both: float32
 // products for float32 queries, at no cost while a KV head has at most 8 rows.
 // With PIECES = 1 a 16-bit q is one float16 (exact: the row is scaled by a power
-// of two first) and p is rounded to 11 bits, below the output's own rounding.
+// of two first) and p is rounded to 11 bits: at most an eighth of a bfloat16
+// output's own rounding, as much as a float16 output's (tq_kv_prompt.cu has figures).
 // The value scale c_b = 2^e_b x mantissa goes with the weights, so that what a row
 // gives no weight, or does not see, costs the rest no bits: m is a power of two at
 // or above 2^(s_t + e_b), p_t = 2^(s_t + e_b - m), the mantissa rides on p in

@@ -12,7 +12,12 @@
 // Codes become float16 once per CTA and position tile (exact), in four warps
 // that go through registers: HBM/L2 -> codes -> float16 -> swizzled operand.
 // Float32 queries take two float16 pieces of q and of p (22 bits): twice the
-// products. 16-bit queries take one.
+// products. 16-bit queries take one, which holds q exactly and rounds p to 11 bits:
+// off by at most 2^-11, an eighth of a bfloat16 output's own rounding and as much
+// as a float16 output's, but averaged over the positions. Against 64 bits the error
+// (2-norm) is 1.7e-3 with one piece or two in bfloat16, 2.3e-4 and 2.1e-4 in
+// float16; two pieces of p cost whole prompts 241 us in place of 211, mixed
+// batches 184 in place of 165 (whole calls).
 //
 // The scales. With a_b, c_b the key and value scale of a 16-position block,
 //   w_t = s_t a_b + log2 c_b,  M >= max w_t - 4 (raised only when w exceeds M + 4),
