@@ -443,7 +443,9 @@ TQ_EXPORT int tq_synth_tokens(int *out, int n, int vocab, uint64_t seed);
  * keys and one for its values: value = code * scale, |code| <= 127.
  * n_layer, n_kv 1 to 65535; hd (head size) a multiple of 8, at most 256; page 16,
  * 32, 64 or 128 tokens; n_pages pages in all, of every layer alike (a page id
- * names the same page in each layer). */
+ * names the same page in each layer). One call takes at most 2^31 - 2^16 - 1 of
+ * anything that it counts: positions of a table row, slots, free pages, tokens to
+ * store, rows (tokens x query heads) to attend (TQ_ERR_UNSUPPORTED). */
 typedef struct {
     int n_layer, n_kv, hd, page, n_pages;
 } tq_kv_config;

@@ -97,6 +97,23 @@ int unaligned(const char *what) {
     return tq_fail(TQ_ERR_ARG, "tensai: %s not aligned to their type", what);
 }
 
+// Indexes in the kernels are int: a position, token or row may be stepped past by a
+// tile, a window or the threads of a cluster, and stays one.
+constexpr int kMostIndex = INT_MAX - 65536;
+
+int check_table(const KvCache &k, const char *what, int cols, int stride) {
+    if (cols < 0 || stride < cols)
+        return tq_fail(TQ_ERR_ARG, "tensai: bad %s table: rows of %d in %d", what, cols, stride);
+    if (cols > kMostIndex / k.c.page)
+        return tq_fail(TQ_ERR_UNSUPPORTED, "tensai: %s table rows of %d pages of %d tokens are too long", what, cols,
+                       k.c.page);
+    return TQ_OK;
+}
+int check_most(const char *what, long long n) {
+    if (n <= kMostIndex) return TQ_OK;
+    return tq_fail(TQ_ERR_UNSUPPORTED, "tensai: %lld %s in one call, at most %d", n, what, kMostIndex);
+}
+
 int bad_pages(const char *what, int n) {
     return tq_fail(TQ_ERR_ARG, "tensai: %s of %d pages: null pointer or negative count", what, n);
 }
@@ -207,9 +224,11 @@ int tq_kv_plan_dev(uint64_t cache, const tq_kv_plan_args *args, void *stream) {
     if (a.n < 0 || a.n > TQ_KV_MAX_REQUESTS)
         return tq_fail(a.n < 0 ? TQ_ERR_ARG : TQ_ERR_UNSUPPORTED, "tensai: a plan takes 0 to %d requests, got %d",
                        TQ_KV_MAX_REQUESTS, a.n);
-    if (a.slots_cap < 0 || a.free_cap < 0 || a.table_cols < 0 || a.table_stride < a.table_cols)
-        return tq_fail(TQ_ERR_ARG, "tensai: bad plan sizes: %d slots, %d free pages, table rows of %d in %d",
-                       a.slots_cap, a.free_cap, a.table_cols, a.table_stride);
+    if (a.slots_cap < 0 || a.free_cap < 0)
+        return tq_fail(TQ_ERR_ARG, "tensai: bad plan sizes: %d slots, %d free pages", a.slots_cap, a.free_cap);
+    if ((rc = check_table(*k, "plan", a.table_cols, a.table_stride)) || (rc = check_most("slots", a.slots_cap)) ||
+        (rc = check_most("free pages", a.free_cap)))
+        return rc;
     if ((a.n && (!a.cached || !a.added || !a.lens || (!a.table && a.table_cols))) || !a.starts || !a.free_count ||
         !a.free_left || (a.free_cap && !a.free_pages) || (a.slots_cap && !a.slots))
         return tq_fail(TQ_ERR_ARG, "tensai: null pointer argument");
@@ -251,9 +270,9 @@ int tq_kv_release_dev(uint64_t cache, const tq_kv_release_args *args, void *stre
     if (a.n < 0 || a.n > TQ_KV_MAX_REQUESTS)
         return tq_fail(a.n < 0 ? TQ_ERR_ARG : TQ_ERR_UNSUPPORTED, "tensai: a release takes 0 to %d requests, got %d",
                        TQ_KV_MAX_REQUESTS, a.n);
-    if (a.free_cap < 0 || a.table_cols < 0 || a.table_stride < a.table_cols)
-        return tq_fail(TQ_ERR_ARG, "tensai: bad release sizes: %d free pages, table rows of %d in %d", a.free_cap,
-                       a.table_cols, a.table_stride);
+    if (a.free_cap < 0) return tq_fail(TQ_ERR_ARG, "tensai: bad release sizes: %d free pages", a.free_cap);
+    if ((rc = check_table(*k, "release", a.table_cols, a.table_stride)) || (rc = check_most("free pages", a.free_cap)))
+        return rc;
     if ((a.n && (!a.done || !a.lens || (!a.table && a.table_cols))) || !a.free_count || !a.free_left ||
         (a.free_cap && !a.free_pages))
         return tq_fail(TQ_ERR_ARG, "tensai: null pointer argument");
@@ -280,6 +299,7 @@ int tq_kv_store_dev(uint64_t cache, int layer, const void *k, const void *v, int
     if (!c || (rc = check_layer(*c, layer)) || (rc = check_dtype(dtype))) return rc;
     const long long row = (long long)c->c.n_kv * c->c.hd;
     if (n < 0) return tq_fail(TQ_ERR_ARG, "tensai: negative token count %d", n);
+    if ((rc = check_most("tokens", n))) return rc;
     if (n && (!k || !v || !slots)) return tq_fail(TQ_ERR_ARG, "tensai: null pointer argument");
     if (n > 1 && (k_stride < row || v_stride < row))
         return tq_fail(TQ_ERR_ARG, "tensai: key and value rows of %lld elements do not fit strides of %lld and %lld",
@@ -316,13 +336,11 @@ int tq_kv_attention_dev(uint64_t cache, int layer, const tq_kv_attention_args *a
                        "tensai: attention takes 0 to %d sequences, got %d (of %d tokens)", TQ_KV_MAX_REQUESTS, a.n,
                        a.n_tokens);
     const long long row = (long long)a.n_q * k->c.hd;
-    if ((long long)a.n_tokens * a.n_q > INT_MAX)
-        return tq_fail(TQ_ERR_UNSUPPORTED, "tensai: %d tokens of %d query heads in one call", a.n_tokens, a.n_q);
+    if ((rc = check_most("rows (tokens x query heads)", (long long)a.n_tokens * a.n_q))) return rc;
     if (a.n_tokens > 1 && (a.q_stride < row || a.out_stride < row))
         return tq_fail(TQ_ERR_ARG, "tensai: query rows of %lld elements do not fit strides of %lld and %lld", row,
                        a.q_stride, a.out_stride);
-    if (a.table_cols < 0 || a.table_stride < a.table_cols || a.table_cols > INT_MAX / k->c.page)
-        return tq_fail(TQ_ERR_ARG, "tensai: bad table rows of %d in %d", a.table_cols, a.table_stride);
+    if ((rc = check_table(*k, "attention", a.table_cols, a.table_stride))) return rc;
     if (!std::isfinite(a.scale)) return tq_fail(TQ_ERR_ARG, "tensai: attention scale is not finite");
     if (a.n == 0 || a.n_tokens == 0) return TQ_OK;
     if (!a.q || !a.out || !a.starts || !a.lens || (!a.table && a.table_cols) || !a.workspace)
