@@ -482,9 +482,12 @@ TQ_EXPORT int tq_kv_status(uint64_t cache, unsigned *bits);
  *   writes slots[t], the place of new token t (tokens of request 0, then 1, ..):
  *     page id * page + offset; entries behind the last token stay as they were.
  * free_left may be free_count, and lens may be cached; other arrays must not
- * overlap. All or nothing: if anything does not fit, a status bit is set, no
- * page is taken, starts are 0, lens = cached and slots[0..slots_cap) = -1, so
- * that a store and an attention behind it do nothing. n <= TQ_KV_MAX_REQUESTS.
+ * overlap. All or nothing: if anything does not fit, or a page that it would
+ * take is outside the cache, a status bit is set, no page is taken, starts are
+ * 0, lens = cached and slots[0..slots_cap) = -1, so that a store and an
+ * attention behind it do nothing. (A table entry of positions held already that
+ * is outside the cache sets TQ_KV_STATUS_PAGE; new tokens of that page alone
+ * have slot -1.) n <= TQ_KV_MAX_REQUESTS.
  * One launch, asynchronous on stream; calls on one free list must not overlap. */
 #define TQ_KV_MAX_REQUESTS 16384
 typedef struct {
@@ -501,7 +504,8 @@ TQ_EXPORT int tq_kv_plan_dev(uint64_t cache, const tq_kv_plan_args *args, void *
 /* Puts the pages of every request with done[i] != 0 back on the free list
  * (free_pages[*free_count + j], requests in order, pages in order) and sets its
  * lens[i] to 0. free_left as in the plan. All or nothing: nothing changes when
- * the list (free_cap entries) cannot take them or a length is bad. */
+ * the list (free_cap entries) cannot take them, a length is bad or a page of
+ * theirs is outside the cache. */
 typedef struct {
     int n, table_stride, table_cols, free_cap;
     const int *done;

@@ -108,6 +108,11 @@ __global__ void __launch_bounds__(kThreads) kv_plan_kernel(tq_kv_plan_args a, in
     if (tokens > a.slots_cap) bad |= TQ_KV_STATUS_SLOTS;
     if (count < 0 || count > a.free_cap) bad |= TQ_KV_STATUS_LENGTH;
     if (pages > count) bad |= TQ_KV_STATUS_POOL;
+    if (count <= a.free_cap && pages <= count) // the ids that the call would take; read again below, near by then
+        for (int j = tid; j < (int)pages; j += kThreads) {
+            const int id = a.free_pages[count - 1 - j];
+            if (id < 0 || id >= n_pages) bad |= TQ_KV_STATUS_PAGE;
+        }
     bad = block_or(bad, &s_bad); // one verdict for the block; every block of the cluster reaches the same one
     if (blocks > 1) cl.barrier_arrive(); // this block has read what may be written in place
     const int g = rank * kThreads + tid, stride = blocks * kThreads;
@@ -134,7 +139,6 @@ __global__ void __launch_bounds__(kThreads) kv_plan_kernel(tq_kv_plan_args a, in
         const int j[1] = {j0}, id = a.free_pages[count - 1 - j0];
         int i[1];
         find_rows(pag, n, j, i);
-        if (id < 0 || id >= n_pages) atomicOr(status, TQ_KV_STATUS_PAGE);
         a.table[(size_t)i[0] * a.table_stride + ((held[i[0]] + P - 1) >> shift) + (j0 - pag[i[0]])] = id;
     }
     for (int t0 = g; t0 < (int)tokens; t0 += kSide * stride) { // slots
@@ -164,12 +168,13 @@ __global__ void __launch_bounds__(kThreads) kv_plan_kernel(tq_kv_plan_args a, in
 __global__ void __launch_bounds__(kThreads) kv_release_kernel(tq_kv_release_args a, int shift, int n_pages,
                                                               unsigned *status) {
     extern __shared__ int sums[]; // [n + 1] page starts of the released requests
+    __shared__ unsigned s_bad_id;
     const int n = a.n, tid = threadIdx.x, P = 1 << shift;
     const int per = (n + kThreads - 1) / kThreads, i0 = min(n, tid * per), i1 = min(n, i0 + per);
     const int count = *a.free_count;
     long long sp = 0, none = 0, pages, unused;
     __shared__ unsigned s_bad;
-    if (tid == 0) s_bad = 0;
+    if (tid == 0) s_bad = s_bad_id = 0;
     unsigned bad = 0;
     for (int i = i0; i < i1; i++) {
         if (!a.done[i]) continue;
@@ -182,27 +187,32 @@ __global__ void __launch_bounds__(kThreads) kv_release_kernel(tq_kv_release_args
     if (count < 0 || count > a.free_cap) bad |= TQ_KV_STATUS_LENGTH;
     if (count + pages > a.free_cap) bad |= TQ_KV_STATUS_POOL;
     bad = block_or(bad, &s_bad);
-    if (bad) {
+    auto refuse = [&]() {
         if (tid == 0) {
             atomicOr(status, bad);
             *a.free_left = count;
         }
-        return;
-    }
+    };
+    if (bad) return refuse();
     for (int i = i0; i < i1; i++) {
         sums[i] = (int)sp;
         if (a.done[i]) sp += (a.lens[i] + P - 1) >> shift;
     }
     if (tid == 0) sums[n] = (int)pages;
     __syncthreads();
-    for (int j = tid; j < (int)pages; j += kThreads) {
+    auto page = [&](int j) { // the j-th released page
         const int x[1] = {j};
         int i[1];
         find_rows(sums, n, x, i);
-        const int id = a.table[(size_t)i[0] * a.table_stride + (j - sums[i[0]])];
-        if (id < 0 || id >= n_pages) atomicOr(status, TQ_KV_STATUS_PAGE);
-        a.free_pages[count + j] = id;
+        return a.table[(size_t)i[0] * a.table_stride + (j - sums[i[0]])];
+    };
+    for (int j = tid; j < (int)pages; j += kThreads) {
+        const int id = page(j);
+        if (id < 0 || id >= n_pages) bad |= TQ_KV_STATUS_PAGE;
     }
+    bad = block_or(bad, &s_bad_id);
+    if (bad) return refuse();
+    for (int j = tid; j < (int)pages; j += kThreads) a.free_pages[count + j] = page(j);
     for (int i = tid; i < n; i += kThreads)
         if (a.done[i]) a.lens[i] = 0;
     if (tid == 0) *a.free_left = count + (int)pages;
