@@ -545,8 +545,9 @@ TQ_EXPORT int tq_kv_store_dev(uint64_t cache, int layer, const void *k, const vo
  * workspace: tq_kv_attention_workspace bytes of device memory, 16-byte
  * aligned, its first TQ_KV_WORKSPACE_HEAD bytes zero before the first call (each
  * call leaves them zero) and never shared by two calls that may overlap (two
- * streams, two graphs replayed at once); calls in order on one stream may share
- * it. n <= TQ_KV_MAX_REQUESTS. Allocates nothing. */
+ * streams, two graphs replayed at once); calls on one stream may share it, from
+ * several threads too where they are of one cache. n <= TQ_KV_MAX_REQUESTS.
+ * Allocates nothing. */
 #define TQ_KV_WORKSPACE_HEAD 4096
 typedef struct {
     const void *q;

@@ -25,6 +25,7 @@ struct KvCache {
     tq_kv_config c{};
     std::vector<TqKvLayer> layers;
     unsigned *status = nullptr;
+    std::mutex launch; // an attention's launches follow one another: threads may share a stream and a workspace
 };
 
 std::mutex g_kv_mu;
@@ -360,6 +361,7 @@ int tq_kv_attention_dev(uint64_t cache, int layer, const tq_kv_attention_args *a
     if (on.err != cudaSuccess) return tq_cuda_fail(on.err, "set device");
     const TqKvAttn t = {a.q,      a.out,  a.dtype, a.q_stride,     a.out_stride, a.n_q,   a.n_tokens,
                         a.n,      a.starts, a.lens, a.table,       a.table_stride, a.table_cols, a.scale, a.workspace};
+    std::lock_guard<std::mutex> lk(k->launch);
     return done(tq_kv_launch_attn(view(*k, layer), t, k->sms, (cudaStream_t)stream), "attention launch");
 }
 
