@@ -80,6 +80,14 @@ class KVCache:
             return self._raw_stream(self._index)
         return self._torch.cuda.current_stream(self.device).cuda_stream
 
+    def _capturing(self, stream) -> bool:
+        """Whether the call's stream is being captured, which need not be the current one."""
+        cuda = self._torch.cuda
+        if stream is None and cuda.current_device() == self._index:
+            return cuda.is_current_stream_capturing()
+        with cuda.stream(cuda.current_stream(self.device) if stream is None else stream):
+            return cuda.is_current_stream_capturing()
+
     def _array(self, name, t, dtype, numel=None):
         if t.dtype is not dtype or not t.is_cuda or t.get_device() != self._index or not t.is_contiguous():
             _refuse(f"{name}: a contiguous {dtype} tensor on {self.device} is required")
@@ -171,7 +179,7 @@ class KVCache:
         tp, ts, tc = self._table(table, n)
         st = self._stream(stream)
         if workspace is None:
-            if torch.cuda.is_current_stream_capturing():
+            if self._capturing(stream):
                 workspace = self.workspace(stream)
             else:
                 workspace = self._spaces.get(st)

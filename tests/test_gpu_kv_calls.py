@@ -44,3 +44,69 @@ def test_threads_on_one_stream():
             t.join()
         assert wrong == [0] * len(qs)
         cache.check()
+
+
+def test_a_captured_call_has_its_own_workspace_whatever_stream_is_current():
+    """Captured through stream=, with another stream current."""
+    rng = np.random.default_rng(52)
+    lens = [5000, 77]
+    cache, ref, table = batch(rng, 2, 64, 64, lens)
+    with cache:
+        qs = [torch.tensor(rng.standard_normal((2, 8, 64)), device="cuda", dtype=torch.float32) for _ in range(2)]
+        args = (cu([0, 1, 2]), cu(lens), cu(table))
+        want = [cache.attention(0, q, *args) for q in qs]
+        made, make = [], cache.workspace
+
+        def workspace(stream=None):
+            w = make(stream)
+            made.append(w.data_ptr())
+            return w
+
+        cache.workspace = workspace
+        side, other = torch.cuda.Stream(), torch.cuda.Stream()
+        torch.cuda.synchronize()
+        cache.attention(0, qs[0], *args, stream=side)  # the stream's own workspace
+        torch.cuda.synchronize()
+        assert len(made) == 1
+        graphs, outs = [], [torch.empty_like(q) for q in qs]
+        for q, out in zip(qs, outs):
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=side):
+                with torch.cuda.stream(other):
+                    cache.attention(0, q, *args, out=out, stream=side)
+            graphs.append(g)
+        assert len(made) == 3 and len(set(made)) == 3
+        streams = [torch.cuda.Stream() for _ in graphs]
+        for _ in range(20):
+            for g, st in zip(graphs, streams):
+                with torch.cuda.stream(st):
+                    g.replay()
+            eager = cache.attention(0, qs[0], *args, stream=side)
+            torch.cuda.synchronize()
+            assert torch.equal(eager, want[0]) and all(torch.equal(x, y) for x, y in zip(outs, want))
+        assert len(made) == 3
+        cache.check()
+
+
+def test_a_stream_is_first_used_in_a_capture():
+    """What the capture made stays the graph's: the stream's eager calls begin
+    with a workspace of their own."""
+    rng = np.random.default_rng(53)
+    lens = [5000, 77]
+    cache, ref, table = batch(rng, 2, 64, 64, lens)
+    with cache:
+        q = torch.tensor(rng.standard_normal((2, 8, 64)), device="cuda", dtype=torch.float32)
+        args = (cu([0, 1, 2]), cu(lens), cu(table))
+        want = cache.attention(0, q, *args)
+        side, other, out = torch.cuda.Stream(), torch.cuda.Stream(), torch.empty_like(q)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            with torch.cuda.stream(other):
+                cache.attention(0, q, *args, out=out, stream=side)
+        assert side.cuda_stream not in cache._spaces
+        eager = cache.attention(0, q, *args, stream=side)
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(eager, want) and torch.equal(out, want)
+        cache.check()
