@@ -449,9 +449,9 @@ __global__ void __launch_bounds__(32 * warps_of(HDP), 1) kv_attn_kernel(const __
             for (int h = 0; h < H; h++) {
                 // a block that the row sees nothing of has the factors of one that is not there: 0 times a NaN is no 0
                 const bool none = !there || pos0 + 16 * t >= lim[h];
-                const float af = none ? 0.f : a * row_unit[h], f = af < kLeast ? kLeast : af; // a NaN stays
+                const float af = none ? 0.f : a * row_unit[h], low = af < kLeast ? kLeast : af; // a NaN stays
                 const float r = none ? 0.f : ride;
-                float v[16], mx = -INFINITY;
+                float f = low, v[16], mx = -INFINITY;
 #pragma unroll
                 for (int j = 0; j < 8; j++)
 #pragma unroll
@@ -466,9 +466,15 @@ __global__ void __launch_bounds__(32 * warps_of(HDP), 1) kv_attn_kernel(const __
                 mx = fmaf(mx, f, lift);
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-                const float m1 = fmaxf(m[h], ceilf(mx)), base = m1 == -INFINITY ? 0.f : m1, off = lift - base;
+                const float m1 = fmaxf(m[h], ceilf(mx)), base = m1 == -INFINITY ? 0.f : m1;
+                float off = lift - base;
                 alpha[h] = ex2(m[h] - base);
                 m[h] = m1;
+                if (fabsf(base) >= kFar) { // m was rounded: so is what it is compared with
+#pragma unroll
+                    for (int j = 0; j < 16; j++) v[j] = __fadd_rn(fmaf(v[j], f, lift), -base);
+                    f = 1.f, off = 0.f;
+                }
                 float sum = 0.f;
 #pragma unroll
                 for (int j = 0; j < 16; j++) {

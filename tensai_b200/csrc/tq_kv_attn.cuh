@@ -48,6 +48,7 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 constexpr float kLeast = 1e-30f; // least score factor of a block: -inf times it stays -inf
+constexpr float kFar = 0x1p20f;  // scores (in powers of two) from which on a weight could leave float16 by their rounding
 constexpr float kLeastValue = 0x1p-92f; // value scales below count as 0: the sums that hold their inverse stay finite
 constexpr float kNoValue = 0x1p-60f;    // what such a scale, of no values, counts as beside others
 

@@ -20,8 +20,8 @@
 // batches 184 in place of 165 (whole calls).
 //
 // The scales. With a_b, c_b the key and value scale of a 16-position block,
-//   w_t = s_t a_b + log2 c_b,  M >= max w_t - 4 (raised only when w exceeds M + 4),
-//   P = 2^(w_t - M + 10),  O = sum P v codes,  L = sum_b (sum P) / c_b,
+//   w_t = s_t a_b + log2 c_b,  M = max w_t - 10 (raised only when w exceeds M + 14),
+//   P = 2^(w_t - M),  O = sum P v codes,  L = sum_b (sum P) / c_b,
 //   out = O / L:
 // the value scale rides in the exponent at no cost, and P stays below 2^14. A
 // block of value scale below 2^-92 counts with c = 2^-60 and zero codes: low enough
@@ -67,8 +67,8 @@ constexpr int kThreads = 32 * (kMmaWarp + 2);
 constexpr int kConsts = 4;      // position tiles whose scales are kept
 constexpr int kSegCost = 2;     // what a segment costs besides its position tiles, in position tiles
 constexpr int kMinUnits = 3;    // units per CTA below which fewer CTAs work
-constexpr float kSlack = 4.f;   // log2 by which w may exceed M
-constexpr float kUnit = 10.f;   // log2 of P at w = M
+constexpr float kUnit = 10.f;   // log2 of P where w is the row's largest
+constexpr float kMostP = 14.f;  // and what it may grow to before M is raised
 constexpr int kJoinThreads = 256, kJoinRows = 32;
 
 constexpr size_t kSharedRoom = 3 * 1024; // struct Shared, behind the operands
@@ -546,9 +546,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const __grid_con
                     *put = top;
                     together();
                     top = fmaxf(top, *get);
-                    if (top > M + kSlack) {
-                        const float alpha = ex2(M - top);
-                        M = top;
+                    if (top - M > kMostP) {
+                        const float next = fabsf(top) >= kFar ? top : top - kUnit; // far: M has no bits for kUnit
+                        const float alpha = ex2(M - next);
+                        M = next;
                         L *= alpha;
                         top = alpha;
                     } else {
@@ -567,15 +568,17 @@ __global__ void __launch_bounds__(kThreads, 1) kv_prompt_kernel(const __grid_con
                         }
                     }
                     // ---- P over S: a block's 8 (or, in two pieces, 16) columns lie in columns already read ----
-                    const float use = M == -INFINITY ? 0.f : M - kUnit;
+                    // w is rounded as the largest was, then M is taken off: from one fused product a large w could
+                    // come out on either side of float16 (fused: 212 us in place of 215, and NaN or 0 from 2^24 on)
+                    const float use = M == -INFINITY ? 0.f : M;
                     over([&](int b, const uint32_t (&v)[16]) {
                         uint32_t y[16];
-                        const float fb = factor(b), ob = sh.lv[cs][b0 + b] - use;
+                        const float fb = factor(b), ob = sh.lv[cs][b0 + b];
                         float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
                         for (int u = 0; u < 16; u += 2) {
                             const float2 s = make_float2(__uint_as_float(v[u]), __uint_as_float(v[u + 1]));
-                            const float2 e = __ffma2_rn(s, make_float2(fb, fb), make_float2(ob, ob));
+                            const float2 e = __fadd2_rn(__ffma2_rn(s, make_float2(fb, fb), make_float2(ob, ob)), make_float2(-use, -use));
                             const float2 x = make_float2(ex2(e.x), ex2(e.y));
                             sum = __fadd2_rn(sum, x);
                             y[u / 2] = pack2(x.x, x.y);
