@@ -375,8 +375,10 @@ TQ_EXPORT int tq_qwen_set_prefill(uint64_t model, int rows);
  * and KV head), a quarter of the memory and of the bytes that a step's attention
  * reads; the prompt and the steps run tq_kv_plan_dev, tq_kv_store_dev and
  * tq_kv_attention_dev, and the generated ids may differ from the parity mode's.
- * The other cache's memory is released. Every rank of a tensor-parallel model
- * calls it alike. */
+ * The other cache's memory is released once the new one is there: while the call
+ * runs both are held, so a context has to fit in float32 first (a cache by itself,
+ * tq_kv_create, has no such need). Every rank of a tensor-parallel model calls it
+ * alike. */
 #define TQ_CACHE_F32 0
 #define TQ_CACHE_INT8 1
 TQ_EXPORT int tq_qwen_set_cache(uint64_t model, int kind);
@@ -547,7 +549,11 @@ TQ_EXPORT int tq_kv_store_dev(uint64_t cache, int layer, const void *k, const vo
  * call leaves them zero) and never shared by two calls that may overlap (two
  * streams, two graphs replayed at once); calls on one stream may share it, from
  * several threads too where they are of one cache. n <= TQ_KV_MAX_REQUESTS.
- * Allocates nothing. */
+ * Allocates nothing.
+ * The host knows no lengths: with enough n_tokens x n_q x table_cols x page (512e6
+ * over the head size, rounded up to 64 or 128) the call first launches the kernel
+ * for sequences of many rows, which costs few rows or short lengths 8 to 28 us.
+ * Tables no wider than the step's longest sequence needs avoid it. */
 #define TQ_KV_WORKSPACE_HEAD 4096
 typedef struct {
     const void *q;
@@ -567,7 +573,9 @@ TQ_EXPORT int tq_kv_attention_dev(uint64_t cache, int layer, const tq_kv_attenti
  * [n][page][n_kv][hd] int8 and scales as [n][n_kv] float32 (load, save), or
  * the values code * scale as [n][page][n_kv][hd] float32 (read). Device
  * memory, asynchronous on stream. load clamps code -128 to -127 and takes a
- * scale that is negative or infinite for NaN. */
+ * scale that is negative or infinite for NaN; no page may occur twice in one
+ * load. What is asked of an id outside the cache is not written
+ * (TQ_KV_STATUS_PAGE). */
 TQ_EXPORT int tq_kv_load_dev(uint64_t cache, int layer, const int *pages, int n, const int8_t *k, const int8_t *v,
                              const float *kscale, const float *vscale, void *stream);
 TQ_EXPORT int tq_kv_save_dev(uint64_t cache, int layer, const int *pages, int n, int8_t *k, int8_t *v, float *kscale,

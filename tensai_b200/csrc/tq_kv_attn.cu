@@ -35,11 +35,12 @@
 //
 // Bound. A sequence or two of ordinary length: latency, 9 us for one tile (the
 // launch; lengths, page, codes one after the other from L2; a first pass through
-// the code), 14 us at 2,559 positions with the joins. Many or long ones: the
+// the code), 13 us at 2,559 positions with the joins. Many or long ones: the
 // instructions between the copies. 64 sequences of 124,000 positions (28 / 4
-// bfloat16 heads of 128) take 39.5 us, 3.2 TB/s (50% of the measured copy), 2
-// sequences of 264,000 64 us, 4.2 TB/s (65%). With two warps a scheduler (248
-// registers, and the rings fill shared memory) issue slots are 31% used; waiting
+// bfloat16 heads of 128) take 39 us, 3.3 TB/s (50% of the measured copy), 2
+// sequences of 264,000 64 us, 4.2 TB/s (64%). With two warps a scheduler (248
+// registers, and the rings fill shared memory; heads above 128 take all 255 and
+// spill 1.2 KB) issue slots are 29% used; waiting
 // for instructions is the largest stall, since a tile's straight code exceeds the
 // instruction caches, then the fixed latency of one instruction after another.
 #include <climits>

@@ -31,8 +31,9 @@
 // its position tiles and kSegCost units before them (its queries come in and its
 // outputs go out), and cut evenly over one CTA per SM. A cut segment's parts go to
 // the workspace; the second kernel joins them in order (the same bits each time).
-// Cost 2: 122 GFLOP of whole prompts take 204 us, mixed sequences of 73 GFLOP 161;
-// cost 1: 226 and 168; 3: 205 and 161; none: 265 and 265.
+// Cost 2: 122 GFLOP of whole prompts took 204 us, mixed sequences of 73 GFLOP 161;
+// cost 1: 226 and 168; 3: 205 and 161; none: 265 and 265. (All before w was rounded
+// apart from its difference to M, as the sides below: 212 and 163 since.)
 //
 // Roles. Two softmax threads a row (211 us; one 217), sixteen warps; four that
 // widen codes (they are busy 60% of the time); one that issues; one that finds
@@ -40,9 +41,9 @@
 // a warp (204 us; by every thread 208).
 //
 // Bound by the chain of one row tile, scores - maximum - exponentials - product,
-// whose parts other tiles only partly cover: whole prompts in bfloat16 run at 597
-// TFLOP/s (36% of the measured matmul rate), the tensor pipe 34%, the exponential
-// unit 35%, issue slots 55% used. Tried: P before the row's maximum is known, in one
+// whose parts other tiles only partly cover: whole prompts in bfloat16 run at 575
+// TFLOP/s (35% of the measured matmul rate), the tensor pipe 32%, the exponential
+// unit 34%, issue slots 55% used. Tried: P before the row's maximum is known, in one
 // pass over S (264 us, its code is too long for the instruction caches), the issuing
 // warp kept together (206), S read 32 columns at a time (204, the same).
 #include <climits>

@@ -18,7 +18,10 @@
 // dimensions a thread, each one 16-byte word.
 //
 // Bound. One token a sequence: latency, 3.8 us for 32 sequences of 4 heads of 128
-// (the slot, the tokens and the scale, the codes of a page that grew). A prompt:
+// (the slot, the tokens and the scale), 4.4 with the pages in 24 caches in turn,
+// 8.3 there if every page's scale grows: its held codes are read, rounded again and
+// written. (A decode step's pages seldom grow: the largest of a page's positions
+// sets its scale.) A prompt:
 // 7,096 bfloat16 tokens of 4 heads of 128 take 21 us for 22 MB, half of it issue
 // slots (a code is about 6 instructions), the rest waiting at the two barriers of
 // a block with 1.3 waves of blocks; 16,000 tokens of 8 float32 heads of 128, 164 MB,
@@ -410,7 +413,7 @@ cudaError_t launch_store(const TqKvView &c, const T *k, const T *v, long long ks
     // Tokens per block, which looks for those that begin a run: a power of two, so that a prompt's
     // pages fall to the blocks evenly, for a few waves of blocks. (One token a block up to 1024:
     // 1000 tokens in a row, 8 heads of 128, bfloat16, pages of 64 took 25.7 us, now 13.1; 300
-    // runs of one 12.3, now 21.)
+    // runs of one 12.3, now 20 to 22.)
     int window = 1;
     while (window < (c.page >= 32 ? 32 : 16) && window * 16ll * sms < n * lines) window *= 2;
     // Threads: 32 elements each of a full page, but 128 for few tokens (100 runs of one, 8 float32

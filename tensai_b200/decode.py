@@ -247,7 +247,8 @@ class Qwen:
 
     def set_cache(self, kind: str) -> None:
         """"float32" (the reference's way, the parity mode) or "int8": the paged
-        8-bit cache, a quarter of the memory (tq_qwen_set_cache)."""
+        8-bit cache, a quarter of the memory once the call is through (it holds
+        both meanwhile; tq_qwen_set_cache)."""
         kinds = {"float32": _lib.TQ_CACHE_F32, "int8": _lib.TQ_CACHE_INT8}
         if kind not in kinds:
             raise ValueError(f'tensai: cache must be "float32" or "int8", got {kind!r}')

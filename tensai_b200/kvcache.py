@@ -165,7 +165,8 @@ class KVCache:
         """softmax(scale q . k) v of the new tokens' queries [tokens][heads][hd]
         over their sequences' cached positions, causal (tq_kv_attention_dev).
         scale: hd ** -0.5 by default. out: a tensor like q; rows behind
-        starts[n] are not written. workspace: self.workspace() by default, one
+        starts[n] are not written. A table wider than the step's longest
+        sequence needs can cost time (the header says when). workspace: self.workspace() by default, one
         for each stream, or one for each call while a graph is captured, so
         that graphs never share one."""
         torch = self._torch
@@ -210,7 +211,7 @@ class KVCache:
     # ---- pages in and out ----
     def load(self, layer: int, pages, k, v, kscale, vscale, stream=None) -> None:
         """Codes [pages][page][n_kv][hd] int8 and scales [pages][n_kv] float32
-        into the listed pages (int32)."""
+        into the listed pages (int32, each once)."""
         torch = self._torch
         pp, n = self._pages(pages)
         m = n * self.n_kv
