@@ -24,7 +24,8 @@ struct KvCache {
     int device = 0, hdp = 0, shift = 0, sms = 0;
     tq_kv_config c{};
     std::vector<TqKvLayer> layers;
-    unsigned *status = nullptr;
+    unsigned *status = nullptr; // TQ_KV_STATUS_* bits, then those last looked at
+    std::mutex look;            // one look at a time
     std::mutex launch; // an attention's launches follow one another: threads may share a stream and a workspace
 };
 
@@ -151,8 +152,8 @@ int tq_kv_create(const tq_kv_config *cfg, uint64_t *cache) {
     const size_t codes = (size_t)bytes, scales = (size_t)c.n_pages * c.n_kv * sizeof(float2);
     cudaError_t e = cudaGetDevice(&k->device);
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&k->sms, cudaDevAttrMultiProcessorCount, k->device);
-    if (e == cudaSuccess) e = tq_dev_malloc((void **)&k->status, sizeof(unsigned));
-    if (e == cudaSuccess) e = cudaMemset(k->status, 0, sizeof(unsigned));
+    if (e == cudaSuccess) e = tq_dev_malloc((void **)&k->status, 2 * sizeof(unsigned));
+    if (e == cudaSuccess) e = cudaMemset(k->status, 0, 2 * sizeof(unsigned));
     for (TqKvLayer &l : k->layers) {
         if (e == cudaSuccess) e = tq_dev_malloc((void **)&l.k, codes);
         if (e == cudaSuccess) e = tq_dev_malloc((void **)&l.v, codes);
@@ -209,10 +210,10 @@ int tq_kv_status(uint64_t cache, unsigned *bits) {
     if (!k) return rc;
     OnDevice on(k->device);
     cudaError_t e = on.err;
+    std::lock_guard<std::mutex> lk(k->look);
     if (e == cudaSuccess) e = cudaDeviceSynchronize();
-    if (e == cudaSuccess) e = cudaMemcpy(bits, k->status, sizeof *bits, cudaMemcpyDeviceToHost);
-    if (e == cudaSuccess && *bits) e = cudaMemset(k->status, 0, sizeof *bits);
-    if (e == cudaSuccess && *bits) e = cudaDeviceSynchronize();
+    if (e == cudaSuccess) e = tq_kv_launch_take(k->status, k->status + 1, nullptr);
+    if (e == cudaSuccess) e = cudaMemcpy(bits, k->status + 1, sizeof *bits, cudaMemcpyDeviceToHost);
     return done(e, "cache status");
 }
 

@@ -56,6 +56,8 @@ __device__ __forceinline__ size_t kv_block_offset(const TqKvView &v, int id, int
 cudaError_t tq_kv_launch_plan(int page_shift, int n_pages, unsigned *status, const tq_kv_plan_args &a, cudaStream_t st);
 cudaError_t tq_kv_launch_release(int page_shift, int n_pages, unsigned *status, const tq_kv_release_args &a,
                                  cudaStream_t st);
+// *bits = *status, and *status = 0, in one step: what other threads' kernels report meanwhile stays.
+cudaError_t tq_kv_launch_take(unsigned *status, unsigned *bits, cudaStream_t st);
 cudaError_t tq_kv_launch_store(const TqKvView &v, const void *k, const void *val, int dtype, long long k_stride,
                                long long v_stride, const long long *slots, int n, int sms, cudaStream_t st);
 // Plain [n][page][n_kv][hd] codes and [n][n_kv] scales <-> the listed pages.

@@ -221,6 +221,8 @@ __global__ void __launch_bounds__(kThreads) kv_release_kernel(tq_kv_release_args
     if (tid == 0) *a.free_left = count + (int)pages;
 }
 
+__global__ void kv_take_kernel(unsigned *status, unsigned *bits) { *bits = atomicExch(status, 0u); }
+
 TqDeviceOnce g_once;
 
 cudaError_t set_up() {
@@ -257,6 +259,11 @@ cudaError_t tq_kv_launch_plan(int page_shift, int n_pages, unsigned *status, con
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     return cudaLaunchKernelEx(&cfg, kv_plan_kernel, a, page_shift, n_pages, status);
+}
+
+cudaError_t tq_kv_launch_take(unsigned *status, unsigned *bits, cudaStream_t st) {
+    kv_take_kernel<<<1, 1, 0, st>>>(status, bits);
+    return cudaGetLastError();
 }
 
 cudaError_t tq_kv_launch_release(int page_shift, int n_pages, unsigned *status, const tq_kv_release_args &a,

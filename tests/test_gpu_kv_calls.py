@@ -110,3 +110,45 @@ def test_a_stream_is_first_used_in_a_capture():
         torch.cuda.synchronize()
         assert torch.equal(eager, want) and torch.equal(out, want)
         cache.check()
+
+
+def test_no_report_is_lost_between_threads():
+    """One thread looks at the status all the time, one makes it report, and what
+    this one makes it report is seen by one of the two that look."""
+    from tensai_b200 import KVCache
+    with KVCache(1, 1, 8, 16, 4) as cache:
+        stop, seen = threading.Event(), []
+
+        def look():
+            while not stop.is_set():
+                seen.append(cache.status())
+
+        def noise():
+            c, a, t, f, k = cu([-1]), cu([1]), cu([[0]]), cu([0]), cu([1])
+            s, ln, sl = cu([0, 0]), cu([0]), torch.zeros(1, dtype=torch.int64, device="cuda")
+            st = torch.cuda.Stream()
+            while not stop.is_set():
+                cache.plan(c, a, t, f, k, s, ln, sl, stream=st)
+                st.synchronize()
+
+        threads = [threading.Thread(target=x) for x in (look, noise)]
+        for t in threads:
+            t.start()
+        lost, bad, mine = 0, cu([9]), torch.cuda.Stream()
+        try:
+            for _ in range(400):
+                at = len(seen)
+                cache.read(0, bad, stream=mine)
+                mine.synchronize()
+                for _ in range(20):
+                    if cache.status() & _lib.TQ_KV_STATUS_PAGE:
+                        break
+                    if any(b & _lib.TQ_KV_STATUS_PAGE for b in seen[at:]):
+                        break
+                else:
+                    lost += 1
+        finally:
+            stop.set()
+            for t in threads:
+                t.join()
+        assert lost == 0
