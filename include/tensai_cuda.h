@@ -455,7 +455,8 @@ typedef struct {
 /* Creates a cache on the thread's current device (tq_set_device): all codes
  * and scales zero. */
 TQ_EXPORT int tq_kv_create(const tq_kv_config *cfg, uint64_t *cache);
-/* Releases a cache (waits for the device first; a second call is a no-op). */
+/* Releases a cache (waits for other threads' calls and the device first; a second
+ * call is a no-op). A captured graph that holds its calls must not run after it. */
 TQ_EXPORT int tq_kv_free(uint64_t cache);
 
 /* Shape and device of a cache. Any output pointer may be NULL. */

@@ -11,6 +11,7 @@
 #include <memory>
 #include <mutex>
 #include <new>
+#include <shared_mutex>
 #include <unordered_map>
 #include <vector>
 
@@ -26,6 +27,8 @@ struct KvCache {
     std::vector<TqKvLayer> layers;
     unsigned *status = nullptr; // TQ_KV_STATUS_* bits, then those last looked at
     std::mutex look;            // one look at a time
+    std::shared_mutex use;      // held by every call up to its last launch; by tq_kv_free alone
+    bool freed = false;
     std::mutex launch; // an attention's launches follow one another: threads may share a stream and a workspace
 };
 
@@ -58,13 +61,30 @@ void release(KvCache &k) {
     k.status = nullptr;
 }
 
-std::shared_ptr<KvCache> find(uint64_t h, int *rc) {
-    std::lock_guard<std::mutex> lk(g_kv_mu);
-    auto it = g_caches.find(h);
+// A cache in use by a call: its memory stays until the call has made its launches.
+struct InUse {
+    std::shared_ptr<KvCache> k; // destroyed after the lock
+    std::shared_lock<std::shared_mutex> lk;
+    explicit operator bool() const { return k != nullptr; }
+    KvCache *operator->() const { return k.get(); }
+    KvCache &operator*() const { return *k; }
+};
+InUse find(uint64_t h, int *rc) {
+    InUse u;
     *rc = TQ_OK;
-    if (it != g_caches.end()) return it->second;
+    {
+        std::lock_guard<std::mutex> lk(g_kv_mu);
+        auto it = g_caches.find(h);
+        if (it != g_caches.end()) u.k = it->second;
+    }
+    if (u) {
+        u.lk = std::shared_lock<std::shared_mutex>(u->use);
+        if (!u->freed) return u;
+        u.lk.unlock();
+        u.k.reset();
+    }
     *rc = tq_fail(TQ_ERR_HANDLE, "tensai: invalid or freed cache handle %llu", (unsigned long long)h);
-    return nullptr;
+    return u;
 }
 
 TqKvView view(const KvCache &k, int layer) {
@@ -187,6 +207,8 @@ int tq_kv_free(uint64_t cache) {
         k = it->second;
         g_caches.erase(it);
     }
+    std::lock_guard<std::shared_mutex> lk(k->use); // calls of other threads have made their launches
+    k->freed = true;
     OnDevice on(k->device);
     cudaDeviceSynchronize(); // no kernel of any stream may still read the pages
     release(*k);

@@ -152,3 +152,42 @@ def test_no_report_is_lost_between_threads():
             for t in threads:
                 t.join()
         assert lost == 0
+
+
+def test_freeing_a_cache_that_other_threads_use():
+    """Calls under way have made their launches before the memory goes; those behind
+    it are errors."""
+    from tensai_b200 import KVCache, TensaiError
+    for turn in range(10):
+        cache = KVCache(1, 1, 64, 16, 64)
+        slots, table = torch.arange(256, device="cuda"), cu(np.arange(64)[None, :])
+        starts, lens = cu([0, 256]), cu([256])
+        started, refused, threads = threading.Barrier(4), [], []
+
+        def work(call):
+            x = torch.randn(256, 1, 64, device="cuda")
+            space = cache.workspace()
+            torch.cuda.synchronize()
+            started.wait()
+            try:
+                for _ in range(100000):
+                    if call == "store":
+                        cache.store(0, x, x, slots)
+                    elif call == "read":
+                        cache.read(0, starts[:1])
+                    else:
+                        cache.attention(0, x, starts, lens, table, workspace=space)
+            except TensaiError as e:
+                refused.append((call, e.code))
+
+        for call in ("store", "read", "attention"):
+            threads.append(threading.Thread(target=work, args=(call,)))
+            threads[-1].start()
+        started.wait()
+        while turn % 2 and cache.status():
+            pass
+        cache.free()
+        for t in threads:
+            t.join()
+        assert sorted(refused) == [(c, _lib.TQ_ERR_HANDLE) for c in ("attention", "read", "store")]
+        torch.cuda.synchronize()
